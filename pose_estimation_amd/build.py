@@ -29,6 +29,7 @@ CXXFLAGS = [
     "-fPIC",
     "-std=c++17",
     "-ffp-contract=off",
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall",
     "-Wno-unused-function",
     f"-I{ROOT / 'include'}",
