@@ -248,6 +248,68 @@ int32_t pe_sgd_step(float* p, float* mom, const float* grad, uint16_t* p_bf16,
                     pe_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * a8. Global gradient norm over many tensors, clipping, and clipped optimizer steps.
+ * Replaces: the gradient transformation between compute_gradients and apply_gradients that
+ * TensorFlow's clip_by_global_norm is for (train.py / model/base_model.py,
+ * PoseEstimation.pyproj:30,34; absent).
+ *
+ *   n = |grad_scale| * sqrt(sum g^2)  (PE_NORM_L2)  or  |grad_scale| * max |g|  (PE_NORM_INF)
+ *   c = n > max_norm ? max_norm / n : 1;      clipped g = g * (grad_scale * c), rounded once
+ * over every element of every tensor.  Squares are summed in float64, so no finite float32
+ * gradient overflows or vanishes; *norm is the float32 value of n.  max_norm may be +inf (never
+ * clips) and 0 (all zero).  If any gradient is NaN or infinite so is n, and every clipped value
+ * is NaN; with skip_nonfinite an optimizer step then changes nothing but *norm.
+ * The order of the sums depends on the lengths alone: the same gradients give the same bits.
+ *
+ * A set of tensors is a DEVICE table of contiguous spans, cut so that workgroup b handles spans
+ * [begin[b], begin[b+1]) (begin: DEVICE array of blocks + 1 entries, blocks <= PE_NORM_MAX_BLOCKS,
+ * the shares about equal).  A span is 1 to 2^62 elements of one type, aligned to its element.
+ * dst is where pe_grad_clip writes (src itself for clipping in place); spans must not overlap
+ * otherwise.  The other calls read src only.
+ *
+ * workspace: pe_grad_norm_workspace_bytes(), 8-byte aligned; calls that share one must be ordered.
+ * ---------------------------------------------------------------------- */
+#define PE_NORM_L2  0
+#define PE_NORM_INF 1
+#define PE_NORM_MAX_BLOCKS 1024
+
+typedef struct pe_grad_span {
+    const void* src;
+    void* dst;
+    int64_t n;
+    int32_t dtype;      /* PE_DTYPE_F32 or PE_DTYPE_BF16 */
+    int32_t reserved;
+} pe_grad_span;
+
+size_t pe_grad_norm_workspace_bytes(void);
+int32_t pe_grad_norm(const pe_grad_span* spans_device, const int32_t* begin_device, int32_t blocks,
+                     int32_t kind, float grad_scale, float* norm, void* workspace,
+                     pe_stream_t stream);
+int32_t pe_grad_clip(const pe_grad_span* spans_device, const int32_t* begin_device, int32_t blocks,
+                     int32_t kind, float grad_scale, double max_norm, float* norm, void* workspace,
+                     pe_stream_t stream);
+
+/* pe_adam_step / pe_sgd_step with clipped gradients: the norm is taken over the set, or over the
+ * step's own arena grad[0..n) when blocks is negative; grad itself is not changed.  Within the
+ * limit the results have the bits of the plain step with the same grad_scale. */
+typedef struct pe_clip_desc {
+    const pe_grad_span* spans;   /* DEVICE table, see above; unused when blocks < 0 */
+    const int32_t* begin;
+    double max_norm;
+    int32_t blocks;
+    int32_t kind;
+    float grad_scale;
+    int32_t skip_nonfinite;
+} pe_clip_desc;
+int32_t pe_adam_clip_step(float* p, float* m, float* v, const float* grad, uint16_t* p_bf16,
+                          int64_t n, float beta1, float beta2, float eps, float step_size,
+                          float denom_scale, const pe_clip_desc* clip, float* norm,
+                          void* workspace, pe_stream_t stream);
+int32_t pe_sgd_clip_step(float* p, float* mom, const float* grad, uint16_t* p_bf16, int64_t n,
+                         float lr, float momentum, const pe_clip_desc* clip, float* norm,
+                         void* workspace, pe_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * a4 / a5. Convolution backbone and deconvolution head (bf16 MFMA implicit GEMM).
  * Replaces: nets/mobilenet_v2.py, model/mobilenet_pose.py, model/base_model.py
  * (PoseEstimation.pyproj:30-32; absent) - the conv / deconv arithmetic the
@@ -642,6 +704,59 @@ int32_t pe_bn_bwd_bf16(const void* da, const void* a, int32_t relu, const void* 
                        const float* act_scale, const float* act_shift, float* dgamma,
                        float* dbeta, void* dz, void* dmasked, void* workspace,
                        int32_t frozen, int32_t* sync, pe_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * a9. Row norm after and before a residual block, fused with the block's gate and residual scale.
+ * Beside pe_bn_*: the norm of a row (the C channels of one pixel or token) needs no batch, so it
+ * serves the batches of two the reference trains with (batch_size 2, test.ipynb:962), batches of
+ * one, and networks whose residual branches start at a small learned scale.
+ * Replaces: the normalisation of nets/mobilenet_v2.py (PoseEstimation.pyproj:32; absent).
+ *
+ *   a = post ? N(y)*post_gamma + post_beta : y
+ *   h = x + scale * phi(gate) * a                 x may be NULL (0)
+ *   z = N(h)*pre_gamma + pre_beta                 only with pre
+ *   N(v) = (v - mean)*rstd (PE_RNORM_LAYER) or v*rstd (PE_RNORM_RMS), over the row,
+ *   rstd = 1/sqrt(mean((v - mean)^2) + eps) (mean 0 for RMS);  phi = identity, sigmoid or silu
+ * y, gate, z and their gradients have y_dtype; x, h and theirs x_dtype: (bf16, bf16),
+ * (bf16, f32) or (f32, f32).  z is the norm of h BEFORE h is rounded.  gammas, betas and scale are
+ * float32 [C] or NULL (1, 0, 1).  gate holds one row for every gate_rows rows of y (1: a row of
+ * its own for each; rows: one for all; must divide rows), or gate_rows = 0.
+ * stats (may be NULL in forward) receives [4][rows] float32: mean, rstd of y, mean, rstd of h;
+ * the planes of a norm that is off, and the means of an RMS norm, are left as they were.
+ * h may be x and z may be y, in place: the same pointer and stride.  C is at most 8192; ld* are
+ * row strides in elements; C % 8 == 0 with every pointer and stride a multiple of 16 bytes is the
+ * fast layout, any other works.
+ *
+ * Backward: from dh (may be NULL: 0) and dz (with pre) to dy, dx (may be NULL), dgate (with a
+ * gate) and the parameter gradients asked for (overwritten, not added to).  dx may be dh, dy may
+ * be dz, in place.  x and y are forward's inputs: h is rebuilt from them in float32.
+ * workspace: pe_rnorm_bwd_workspace_bytes(d), 16-byte aligned, needed for parameter gradients
+ * and for a gate shared by several rows.  The sums' order depends on the sizes alone.
+ * ---------------------------------------------------------------------- */
+#define PE_RNORM_LAYER 0
+#define PE_RNORM_RMS   1
+#define PE_GATE_NONE    0
+#define PE_GATE_SIGMOID 1
+#define PE_GATE_SILU    2
+
+typedef struct pe_rnorm_desc {
+    int64_t rows, gate_rows;
+    int64_t ldy, ldx, ldgate, ldh, ldz;            /* forward */
+    int64_t lddh, lddz, lddy, lddx, lddgate;       /* backward */
+    int32_t C, y_dtype, x_dtype, norm, post, pre, gate_act;
+    float eps;
+} pe_rnorm_desc;
+int32_t pe_rnorm_fwd(const pe_rnorm_desc* d, const void* y, const void* x, const float* post_gamma,
+                     const float* post_beta, const float* scale, const void* gate,
+                     const float* pre_gamma, const float* pre_beta, void* h, void* z,
+                     float* stats, pe_stream_t stream);
+size_t pe_rnorm_bwd_workspace_bytes(const pe_rnorm_desc* d);
+int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const void* dz, const void* y,
+                     const void* x, const float* stats, const float* post_gamma,
+                     const float* post_beta, const float* scale, const void* gate,
+                     const float* pre_gamma, void* dy, void* dx, void* dgate, float* dpost_gamma,
+                     float* dpost_beta, float* dscale, float* dpre_gamma, float* dpre_beta,
+                     void* workspace, size_t workspace_bytes, pe_stream_t stream);
 
 /* Folded constants of batch-norm layers that run on their running statistics (inference, or
  * training with frozen statistics), for any number of layers in one launch:

@@ -7,10 +7,13 @@ the first op does, and fails loudly if it has not been built
 """
 from . import _ffi  # noqa: F401
 from .ops import (  # noqa: F401
+    GradSet,
     adam_scalars,
     adam_step,
+    clip_grads,
     decode,
     gaussian_table,
+    grad_norm,
     mse_fwd_bwd,
     mse_workspace,
     render_targets,

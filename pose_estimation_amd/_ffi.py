@@ -6,7 +6,7 @@ an instruction to build it, and every op raises if its tensors are not on a GPU.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libpe_hip.so"
@@ -17,6 +17,9 @@ PE_E_HIP = -2
 PE_E_UNSUPPORTED = -3
 PE_DTYPE_F32 = 0
 PE_DTYPE_BF16 = 1
+PE_NORM_L2 = 0
+PE_NORM_INF = 1
+PE_NORM_MAX_BLOCKS = 1024
 PE_MAX_RADIUS = 31
 PE_MSE_STATIC_MAX_MAPS = 65536
 
@@ -85,6 +88,21 @@ SIGNATURES = {
         c_int32,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_float, c_float, c_float, c_void_p],
     ),
+    "pe_grad_norm_workspace_bytes": (c_size_t, []),
+    "pe_grad_norm": (
+        c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p]),
+    "pe_grad_clip": (
+        c_int32,
+        [c_void_p, c_void_p, c_int32, c_int32, c_float, c_double, c_void_p, c_void_p, c_void_p]),
+    "pe_adam_clip_step": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+         c_float, c_float, c_float, c_float, c_float, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "pe_sgd_clip_step": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_float, c_float, c_void_p, c_void_p,
+         c_void_p, c_void_p]),
     "pe_conv2d_fwd_bf16": (
         c_int32,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
@@ -263,6 +281,9 @@ SIGNATURES = {
     "pe_bn_finalize_apply_bf16": (
         c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_float,
                   c_float] + [c_void_p] * 7 + [c_int32, c_void_p, c_void_p, c_void_p]),
+    "pe_rnorm_fwd": (c_int32, [c_void_p] * 13),
+    "pe_rnorm_bwd_workspace_bytes": (c_size_t, [c_void_p]),
+    "pe_rnorm_bwd": (c_int32, [c_void_p] * 20 + [c_size_t, c_void_p]),
     "pe_bn_fold_f32": (c_int32, [c_void_p, c_int32, c_float, c_void_p]),
 }
 
@@ -279,6 +300,27 @@ class ConvStage(ctypes.Structure):
 
     _fields_ = [("desc", ConvDesc), ("w", c_void_p), ("scale", c_void_p), ("shift", c_void_p),
                 ("residual", c_void_p), ("y", c_void_p)]
+
+
+class ClipDesc(ctypes.Structure):
+    """Mirror of pe_clip_desc (include/pe_api.h)."""
+
+    _fields_ = [("spans", c_void_p), ("begin", c_void_p), ("max_norm", c_double),
+                ("blocks", c_int32), ("kind", c_int32), ("grad_scale", c_float),
+                ("skip_nonfinite", c_int32)]
+
+
+PE_RNORM_LAYER, PE_RNORM_RMS = 0, 1
+PE_GATE_NONE, PE_GATE_SIGMOID, PE_GATE_SILU = 0, 1, 2
+
+
+class RnormDesc(ctypes.Structure):
+    """Mirror of pe_rnorm_desc (include/pe_api.h)."""
+
+    _fields_ = [(n, c_int64) for n in ("rows", "gate_rows", "ldy", "ldx", "ldgate", "ldh", "ldz",
+                                       "lddh", "lddz", "lddy", "lddx", "lddgate")] + \
+               [(n, c_int32) for n in ("C", "y_dtype", "x_dtype", "norm", "post", "pre",
+                                       "gate_act")] + [("eps", c_float)]
 
 
 PE_CONV_MAX_CHAIN = 3

@@ -47,6 +47,10 @@ DEFAULTS: Dict[str, Dict[str, Any]] = {
         "learning_rate_decay": {"decay_rate": 0.95, "decay_steps": 10000},
         "optimizer": {"name": "adam",
                       "params": {"beta1": 0.9, "beta2": 0.999, "epsilon": "1e-8"}},
+        # limit of the gradients' global norm over all parameters (None: no clipping), and whether
+        # a step whose norm is not finite leaves the parameters as they are
+        "gradient_clip_norm": None,
+        "skip_nonfinite_steps": False,
         "preprocess": {"image_resize": [256, 192]},
         # the reference trains with {"flip_left_right": True, "random_crop": True,
         # "scale_range": [0.5, 2.0]} (test.ipynb:995-997); None = frames are fed as they are

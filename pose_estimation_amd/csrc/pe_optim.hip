@@ -7,6 +7,7 @@
 #include <math.h>
 
 #include "pe_common.h"
+#include "pe_gradnorm.h"
 
 namespace pe {
 
@@ -104,6 +105,145 @@ __global__ __launch_bounds__(256) void sgd_kernel(float* __restrict__ p, float* 
     }
 }
 
+// The clipped steps: the factor of the gradients comes from the partial results of a norm that the
+// launch before has left in memory, so the clipped gradient is never stored and the arena is read
+// once more for the norm, not twice.  Each workgroup folds the partials for itself; 2048 of them
+// keep that at a thousandth of the traffic.  The factor multiplies in float64 and rounds once, so
+// a step whose norm is within the limit has the bits of the plain step.
+struct ClipStep {
+    const double* part;
+    int parts;
+    ClipRule rule;
+    int skip_nonfinite;
+    float* norm;
+    // The gradients' factor; false: the norm is not finite and the step is to be skipped.
+    __device__ __forceinline__ bool factor(double& f) const {
+        const double n = norm_fold(part, parts, rule);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+        f = clip_factor(n, rule);
+        return !(skip_nonfinite && !isfinite(n));
+    }
+};
+
+__global__ __launch_bounds__(256) void adam_clip_kernel(float* __restrict__ p, float* __restrict__ m,
+                                                        float* __restrict__ v,
+                                                        const float* __restrict__ grad,
+                                                        uint16_t* __restrict__ pb, long n,
+                                                        AdamHyper h, ClipStep c) {
+    double f;
+    if (!c.factor(f)) return;
+    const long n4 = n >> 2;
+    const long tid = (long)blockIdx.x * 256 + threadIdx.x;
+    const long nth = (long)gridDim.x * 256;
+    float4* p4 = reinterpret_cast<float4*>(p);
+    float4* m4 = reinterpret_cast<float4*>(m);
+    float4* v4 = reinterpret_cast<float4*>(v);
+    const f32x4* g4 = reinterpret_cast<const f32x4*>(grad);
+    uint2* pb4 = reinterpret_cast<uint2*>(pb);
+    for (long i = tid; i < n4; i += nth) {
+        float4 pp = p4[i], mm = m4[i], vv = v4[i];
+        const f32x4 gg = __builtin_nontemporal_load(g4 + i);
+        adam_one(pp.x, mm.x, vv.x, scaled(gg.x, f), h);
+        adam_one(pp.y, mm.y, vv.y, scaled(gg.y, f), h);
+        adam_one(pp.z, mm.z, vv.z, scaled(gg.z, f), h);
+        adam_one(pp.w, mm.w, vv.w, scaled(gg.w, f), h);
+        p4[i] = pp;
+        m4[i] = mm;
+        v4[i] = vv;
+        if (pb) {
+            uint2 o;
+            o.x = pack_bf16x2_bits(pp.x, pp.y);
+            o.y = pack_bf16x2_bits(pp.z, pp.w);
+            pb4[i] = o;
+        }
+    }
+    for (long i = n4 * 4 + tid; i < n; i += nth) {
+        float pp = p[i], mm = m[i], vv = v[i];
+        adam_one(pp, mm, vv, scaled(grad[i], f), h);
+        p[i] = pp;
+        m[i] = mm;
+        v[i] = vv;
+        if (pb) pb[i] = (uint16_t)float_to_bf16_bits(pp);
+    }
+}
+
+__global__ __launch_bounds__(256) void sgd_clip_kernel(float* __restrict__ p, float* __restrict__ mom,
+                                                       const float* __restrict__ grad,
+                                                       uint16_t* __restrict__ pb, long n, float lr,
+                                                       float momentum, ClipStep c) {
+    double f;
+    if (!c.factor(f)) return;
+    const long n4 = n >> 2;
+    const long tid = (long)blockIdx.x * 256 + threadIdx.x;
+    const long nth = (long)gridDim.x * 256;
+    float4* p4 = reinterpret_cast<float4*>(p);
+    float4* m4 = reinterpret_cast<float4*>(mom);
+    const f32x4* g4 = reinterpret_cast<const f32x4*>(grad);
+    uint2* pb4 = reinterpret_cast<uint2*>(pb);
+    auto one = [&](float& pp, float& mm, float g) {
+        mm = momentum * mm + g;
+        pp = pp - lr * mm;
+    };
+    for (long i = tid; i < n4; i += nth) {
+        float4 pp = p4[i], mm = m4[i];
+        const f32x4 gg = __builtin_nontemporal_load(g4 + i);
+        one(pp.x, mm.x, scaled(gg.x, f));
+        one(pp.y, mm.y, scaled(gg.y, f));
+        one(pp.z, mm.z, scaled(gg.z, f));
+        one(pp.w, mm.w, scaled(gg.w, f));
+        p4[i] = pp;
+        m4[i] = mm;
+        if (pb) {
+            uint2 o;
+            o.x = pack_bf16x2_bits(pp.x, pp.y);
+            o.y = pack_bf16x2_bits(pp.z, pp.w);
+            pb4[i] = o;
+        }
+    }
+    for (long i = n4 * 4 + tid; i < n; i += nth) {
+        float pp = p[i], mm = mom[i];
+        one(pp, mm, scaled(grad[i], f));
+        p[i] = pp;
+        mom[i] = mm;
+        if (pb) pb[i] = (uint16_t)float_to_bf16_bits(pp);
+    }
+}
+
+static unsigned clip_grid(long n) {
+    long blocks = ((n >> 2) + 255) / 256;
+    if (blocks < 1) blocks = 1;
+    if (blocks > 2048) blocks = 2048;
+    return (unsigned)blocks;
+}
+
+// Checks the clipping arguments and enqueues the norm: over the given set, or (blocks < 0) over
+// the step's own gradient arena.
+static int32_t start_clip(const char* what, const float* grad, int64_t n, const pe_clip_desc* d,
+                          float* norm, void* workspace, pe_stream_t stream, ClipStep* c) {
+    PE_REQUIRE(d, PE_E_INVALID, "%s: NULL clip description", what);
+    PE_REQUIRE(d->max_norm >= 0.0, PE_E_INVALID, "%s: max_norm must not be negative or NaN", what);
+    PE_REQUIRE(isfinite(d->grad_scale), PE_E_INVALID, "%s: grad_scale must be finite", what);
+    PE_REQUIRE(d->kind == PE_NORM_L2 || d->kind == PE_NORM_INF, PE_E_UNSUPPORTED,
+               "%s: unknown norm %d", what, d->kind);
+    PE_REQUIRE(d->blocks <= kNormMaxParts, PE_E_INVALID, "%s: %d workgroups, at most %d", what,
+               d->blocks, kNormMaxParts);
+    PE_REQUIRE(d->blocks <= 0 || (d->spans && d->begin), PE_E_INVALID, "%s: NULL table", what);
+    PE_REQUIRE(norm && workspace, PE_E_INVALID, "%s: NULL norm or workspace", what);
+    PE_REQUIRE(aligned(workspace, 8), PE_E_INVALID, "%s: workspace must be 8-byte aligned", what);
+    double* part = static_cast<double*>(workspace);
+    c->part = part;
+    c->rule = ClipRule{(double)d->grad_scale, d->max_norm, d->kind};
+    c->skip_nonfinite = d->skip_nonfinite;
+    c->norm = norm;
+    if (d->blocks >= 0) {
+        c->parts = d->blocks;
+        launch_norm_parts(d->spans, d->begin, d->blocks, d->kind, part, as_stream(stream));
+    } else {
+        launch_flat_norm(grad, (long)n, d->kind, part, &c->parts, as_stream(stream));
+    }
+    return PE_OK;
+}
+
 static unsigned optim_grid(long n) {
     long blocks = ((n >> 2) + 255) / 256;
     if (blocks < 1) blocks = 1;
@@ -148,4 +288,48 @@ extern "C" int32_t pe_sgd_step(float* p, float* mom, const float* grad, uint16_t
     pe::launch(sgd_kernel, optim_grid(n), 256, 0, as_stream(stream), p, mom, grad, p_bf16, (long)n, lr,
                                                             momentum, grad_scale);
     return check_launch("pe_sgd_step");
+}
+
+extern "C" int32_t pe_adam_clip_step(float* p, float* m, float* v, const float* grad,
+                                     uint16_t* p_bf16, int64_t n, float beta1, float beta2,
+                                     float eps, float step_size, float denom_scale,
+                                     const pe_clip_desc* clip, float* norm, void* workspace,
+                                     pe_stream_t stream) {
+    using namespace pe;
+    PE_REQUIRE(n >= 0, PE_E_INVALID, "pe_adam_clip_step: negative n");
+    PE_REQUIRE(n == 0 || (p && m && v && grad), PE_E_INVALID, "pe_adam_clip_step: NULL arena pointer");
+    PE_REQUIRE(aligned(p, 16) && aligned(m, 16) && aligned(v, 16) && aligned(grad, 16) &&
+                   aligned(p_bf16, 8),
+               PE_E_INVALID, "pe_adam_clip_step: arenas must be 16-byte aligned (bf16 copy: 8)");
+    ClipStep c;
+    const int32_t bad = start_clip("pe_adam_clip_step", grad, n, clip, norm, workspace, stream, &c);
+    if (bad) return bad;
+    AdamHyper h;
+    h.beta1 = beta1;
+    h.beta2 = beta2;
+    h.omb1 = (float)(1.0 - (double)beta1);
+    h.omb2 = (float)(1.0 - (double)beta2);
+    h.eps = eps;
+    h.step_size = step_size;
+    h.denom_scale = denom_scale;
+    h.grad_scale = 1.0f;   // part of the factor
+    pe::launch(adam_clip_kernel, clip_grid(n), 256, 0, as_stream(stream), p, m, v, grad, p_bf16,
+               (long)n, h, c);
+    return check_launch("pe_adam_clip_step");
+}
+
+extern "C" int32_t pe_sgd_clip_step(float* p, float* mom, const float* grad, uint16_t* p_bf16,
+                                    int64_t n, float lr, float momentum, const pe_clip_desc* clip,
+                                    float* norm, void* workspace, pe_stream_t stream) {
+    using namespace pe;
+    PE_REQUIRE(n >= 0, PE_E_INVALID, "pe_sgd_clip_step: negative n");
+    PE_REQUIRE(n == 0 || (p && mom && grad), PE_E_INVALID, "pe_sgd_clip_step: NULL arena pointer");
+    PE_REQUIRE(aligned(p, 16) && aligned(mom, 16) && aligned(grad, 16) && aligned(p_bf16, 8),
+               PE_E_INVALID, "pe_sgd_clip_step: arenas must be 16-byte aligned (bf16 copy: 8)");
+    ClipStep c;
+    const int32_t bad = start_clip("pe_sgd_clip_step", grad, n, clip, norm, workspace, stream, &c);
+    if (bad) return bad;
+    pe::launch(sgd_clip_kernel, clip_grid(n), 256, 0, as_stream(stream), p, mom, grad, p_bf16, (long)n,
+               lr, momentum, c);
+    return check_launch("pe_sgd_clip_step");
 }

@@ -142,6 +142,7 @@ class TrainGraph:
         self.opt_m = torch.zeros(off, dtype=torch.float32, device=dev)
         self.opt_v = torch.zeros(off, dtype=torch.float32, device=dev)
         self.step_count = 0
+        self.grad_norm: Optional[torch.Tensor] = None   # of the last clipped step
         bn_layers = [L for L in self.layers if L.kind != "head"]
         self.bn_mean = {L.name: torch.zeros(L.cout, device=dev) for L in bn_layers}
         self.bn_var = {L.name: torch.ones(L.cout, device=dev) for L in bn_layers}
@@ -652,18 +653,25 @@ class TrainGraph:
 
     # ------------------------------------------------------------------ optimizer
     def optimizer_step(self, lr: float, optimizer: str = "adam", beta1: float = 0.9,
-                       beta2: float = 0.999, eps: float = 1e-8, momentum: float = 0.9) -> None:
+                       beta2: float = 0.999, eps: float = 1e-8, momentum: float = 0.9,
+                       clip_norm: Optional[float] = None, skip_nonfinite: bool = False) -> None:
+        """clip_norm: limit of the gradients' global norm, taken after the exchange, so that every
+        rank clips alike; self.grad_norm is then the norm before clipping ([1], on the device).
+        skip_nonfinite: leave everything as it is when that norm is not finite."""
         scale = 1.0
         if self.bucketer is not None:
             self.bucketer.finish()
             scale = self.bucketer.grad_scale
         self.step_count += 1
         if optimizer == "adam":
-            ops.adam_step(self.master, self.opt_m, self.opt_v, self.grads, self.step_count, lr,
-                          beta1, beta2, eps, p_bf16=self.work, tf1=True, grad_scale=scale)
+            self.grad_norm = ops.adam_step(self.master, self.opt_m, self.opt_v, self.grads,
+                                           self.step_count, lr, beta1, beta2, eps,
+                                           p_bf16=self.work, tf1=True, grad_scale=scale,
+                                           max_norm=clip_norm, skip_nonfinite=skip_nonfinite)
         elif optimizer == "sgd":
-            ops.sgd_step(self.master, self.opt_m, self.grads, lr, momentum, p_bf16=self.work,
-                         grad_scale=scale)
+            self.grad_norm = ops.sgd_step(self.master, self.opt_m, self.grads, lr, momentum,
+                                          p_bf16=self.work, grad_scale=scale, max_norm=clip_norm,
+                                          skip_nonfinite=skip_nonfinite)
         else:
             raise ValueError(f"unknown optimizer {optimizer!r}")
         self.refresh_transposes()

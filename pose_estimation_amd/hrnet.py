@@ -554,11 +554,12 @@ class TrainablePoseHRNet(TrainGraph):
                    lr: float = 1e-3, optimizer: str = "adam", beta1: float = 0.9,
                    beta2: float = 0.999, eps: float = 1e-8, momentum: float = 0.9,
                    x_s2d: Optional[torch.Tensor] = None, hip_graph: bool = False,
-                   host_replay: bool = False):
+                   host_replay: bool = False, clip_norm: Optional[float] = None,
+                   skip_nonfinite: bool = False):
         """One optimisation step; returns (loss [1] device tensor, per_joint [K]).  hip_graph:
         replay the forward/loss/backward pass as one captured HIP graph (see TrainGraph.replay);
         host_replay: enqueue it from the call list recorded on the first step
-        (TrainGraph.replay_host)."""
+        (TrainGraph.replay_host); clip_norm, skip_nonfinite: see TrainGraph.optimizer_step."""
         fn, x = (self._pass, x_s2d) if x_s2d is not None else (self._pass_u8, images_u8)
         if host_replay:
             loss, per_joint = self.replay_host(fn, x, joints, mask)
@@ -566,5 +567,5 @@ class TrainablePoseHRNet(TrainGraph):
             loss, per_joint = self.replay(fn, x, joints, mask)
         else:
             loss, per_joint = fn(x, joints, mask)
-        self.optimizer_step(lr, optimizer, beta1, beta2, eps, momentum)
+        self.optimizer_step(lr, optimizer, beta1, beta2, eps, momentum, clip_norm, skip_nonfinite)
         return loss, per_joint

@@ -459,12 +459,14 @@ class TrainablePoseMobileNetV2(TrainGraph):
                    lr: float = 1e-3, optimizer: str = "adam", beta1: float = 0.9,
                    beta2: float = 0.999, eps: float = 1e-8, momentum: float = 0.9,
                    x_s2d: Optional[torch.Tensor] = None, hip_graph: bool = False,
-                   det_labels=None, host_replay: bool = False):
+                   det_labels=None, host_replay: bool = False, clip_norm: Optional[float] = None,
+                   skip_nonfinite: bool = False):
         """One optimisation step on heat-map loss + vector-map loss (+ objectness and box loss
         with the detection branch, which needs det_labels = (classes, weights, regs)); returns
         (loss [1] device tensor, per_joint [K]).  hip_graph: replay the forward/loss/backward
         pass as one captured HIP graph (see TrainGraph.replay); host_replay: enqueue it from the
-        call list recorded on the first step (TrainGraph.replay_host)."""
+        call list recorded on the first step (TrainGraph.replay_host); clip_norm, skip_nonfinite:
+        see TrainGraph.optimizer_step."""
         fn, x = (self._pass, x_s2d) if x_s2d is not None else (self._pass_u8, images_u8)
         if hip_graph or host_replay:
             if self.det_blocks:
@@ -473,5 +475,5 @@ class TrainablePoseMobileNetV2(TrainGraph):
             loss, per_joint = run(fn, x, joints, mask)
         else:
             loss, per_joint = fn(x, joints, mask, det_labels)
-        self.optimizer_step(lr, optimizer, beta1, beta2, eps, momentum)
+        self.optimizer_step(lr, optimizer, beta1, beta2, eps, momentum, clip_norm, skip_nonfinite)
         return loss, per_joint

@@ -14,8 +14,9 @@ from typing import Optional
 import numpy as np
 import torch
 
-from ._ffi import (PE_CONV_MAX_CHAIN, PE_WGRAD_MAX_BATCH, ConvDesc, ConvStage, WgradJob, check,
-                   lib)
+from ._ffi import (PE_CONV_MAX_CHAIN, PE_DTYPE_BF16, PE_DTYPE_F32, PE_GATE_NONE, PE_GATE_SIGMOID,
+                   PE_GATE_SILU, PE_RNORM_LAYER, PE_RNORM_RMS, PE_WGRAD_MAX_BATCH, ConvDesc,
+                   ConvStage, RnormDesc, WgradJob, check, lib)
 from .ops import _need_gpu, _ptr, _stream, on_device
 
 BF16 = torch.bfloat16
@@ -1308,3 +1309,236 @@ def bn_bwd(da: torch.Tensor, a: Optional[torch.Tensor], z: torch.Tensor, gamma, 
                                    dbeta.data_ptr(), dz.data_ptr(), _ptr(g), ws.data_ptr(),
                                    int(bool(frozen)), _ptr(sync), _stream(z)))
     return dz, g
+
+
+# --------------------------------------------------------------------------- row norm of a block
+RNORM_MAX_C = 8192
+_RNORM_KIND = {"layer": PE_RNORM_LAYER, "rms": PE_RNORM_RMS}
+_GATE_ACT = {"none": PE_GATE_NONE, "sigmoid": PE_GATE_SIGMOID, "silu": PE_GATE_SILU}
+_RNORM_DTYPE = {torch.float32: PE_DTYPE_F32, torch.bfloat16: PE_DTYPE_BF16}
+
+
+def _row_stride(t: torch.Tensor, name: str) -> int:
+    """Elements from one row (last dimension) to the next; rows must be evenly spaced."""
+    if t.is_contiguous():
+        return t.shape[-1]
+    shape, strides = t.shape, t.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name}: channels must be adjacent in memory, strides {strides}")
+    ld = span = None
+    for size, stride in zip(shape[-2::-1], strides[-2::-1]):
+        if size == 1:
+            continue
+        if ld is None:
+            ld = stride
+        elif stride != span:
+            raise ValueError(f"{name}: rows must be evenly spaced, strides {strides}")
+        span = stride * size
+    return shape[-1] if ld is None else ld
+
+
+def _channel_vector(t: Optional[torch.Tensor], C: int, device, name: str):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != C or not t.is_contiguous() or \
+            t.device != device:
+        raise ValueError(f"{name} must be contiguous float32 [{C}] on {device}")
+    return t.data_ptr()
+
+
+def _block_norm_desc(y, x, gate, gate_act, norm, post, pre, eps) -> RnormDesc:
+    """Checks what both directions take and describes it."""
+    _need_gpu(y, x, gate)
+    if y.dim() < 1 or not 1 <= y.shape[-1] <= RNORM_MAX_C:
+        raise ValueError(f"y must be [..., C] with 1 to {RNORM_MAX_C} channels, "
+                         f"got {tuple(y.shape)}")
+    C = y.shape[-1]
+    rows = y.numel() // C
+    yt = _RNORM_DTYPE.get(y.dtype)
+    xt = yt if x is None else _RNORM_DTYPE.get(x.dtype)
+    if yt is None or xt is None or (yt == PE_DTYPE_F32 and xt != PE_DTYPE_F32):
+        raise ValueError("y and x must be bfloat16 or float32, x float32 where y is: got "
+                         f"{y.dtype}, {None if x is None else x.dtype}")
+    if norm not in _RNORM_KIND:
+        raise ValueError(f"unknown norm {norm!r}")
+    if gate_act not in _GATE_ACT:
+        raise ValueError(f"unknown gate activation {gate_act!r}")
+    if not 0.0 < eps < float("inf"):
+        raise ValueError(f"eps must be positive, got {eps}")
+    d = RnormDesc(rows=rows, C=C, y_dtype=yt, x_dtype=xt, norm=_RNORM_KIND[norm],
+                  post=post is not None, pre=pre is not None, gate_act=_GATE_ACT[gate_act],
+                  eps=eps, ldy=_row_stride(y, "y"))
+    if x is not None:
+        if x.shape != y.shape or x.device != y.device:
+            raise ValueError(f"x must be {tuple(y.shape)} on {y.device}, "
+                             f"got {tuple(x.shape)} on {x.device}")
+        d.ldx = _row_stride(x, "x")
+    if gate is None:
+        if gate_act != "none":
+            raise ValueError("gate_act without a gate")
+        return d
+    if gate.dtype != y.dtype or gate.device != y.device or gate.dim() < 1 or gate.shape[-1] != C:
+        raise ValueError(f"gate must be {y.dtype} with {C} channels on {y.device}")
+    G = gate.numel() // C
+    if gate.shape != y.shape and (gate.dim() > 2 or (rows % G if G else rows)):
+        raise ValueError(f"gate {tuple(gate.shape)} is neither of y's shape {tuple(y.shape)}, nor "
+                         "[C], nor [G, C] with G equal runs of rows")
+    d.gate_rows = rows // G if G else 0
+    d.ldgate = _row_stride(gate, "gate")
+    return d
+
+
+def _memory(t: torch.Tensor, ld: int):
+    size, C = t.element_size(), t.shape[-1]
+    rows = t.numel() // C
+    return t.data_ptr(), ((rows - 1) * ld + C) * size, ld * size, C * size
+
+
+def _refuse_overlap(a: torch.Tensor, lda: int, b: Optional[torch.Tensor], ldb: int, what: str,
+                    in_place: bool) -> None:
+    """a is written: b may share no element with it, or (in_place) be exactly it."""
+    if b is None or a.numel() == 0 or b.numel() == 0:
+        return
+    (pa, na, la, ca), (pb, nb, lb, cb) = _memory(a, lda), _memory(b, ldb)
+    if pa + na <= pb or pb + nb <= pa:
+        return
+    if in_place and pa == pb and la == lb and a.dtype == b.dtype:
+        return
+    if la == lb and la > 0:                  # side by side in wider rows
+        off = (pb - pa) % la
+        if ca <= off and off + cb <= la:
+            return
+    raise ValueError(f"{what} share memory")
+
+
+def residual_norm(y: torch.Tensor, x: Optional[torch.Tensor] = None, *, norm: str = "layer",
+                  post=None, pre=None, scale: Optional[torch.Tensor] = None,
+                  gate: Optional[torch.Tensor] = None, gate_act: str = "none",
+                  eps: float = 1e-6, want_stats: bool = False, out=None):
+    """End of a residual block and start of the next one, in one launch -> (h, z, stats):
+
+        h = x + scale * act(gate) * N(y) ;   z = N(h)        N over the last dimension of a row
+
+    y [..., C]: what the block computed, x (same shape, or None for 0): the residual stream;
+    bfloat16 or float32 (x may be float32 beside bfloat16 y; h has x's type, z has y's).
+    post / pre: the norm of y / of h as a pair (gamma, beta) of float32 [C] vectors, each of
+    which may be None; None = no such norm (without `pre`, z is None).  norm: "layer" or "rms".
+    scale: float32 [C].  gate (y's type): y's shape, or [G, C] for G equal runs of consecutive
+    rows (one per image, say), or [C]; gate_act "none", "sigmoid" or "silu".
+    want_stats: also return the float32 [4, rows] statistics residual_norm_bwd needs.
+    out = (h, z): where to write; h may be x and z may be y, in place.  Rows may be strided."""
+    d = _block_norm_desc(y, x, gate, gate_act, norm, post, pre, eps)
+    C, rows, dev = d.C, d.rows, y.device
+    gp = bp = gq = bq = None
+    if post is not None:
+        gp = _channel_vector(post[0], C, dev, "post gamma")
+        bp = _channel_vector(post[1], C, dev, "post beta")
+    if pre is not None:
+        gq = _channel_vector(pre[0], C, dev, "pre gamma")
+        bq = _channel_vector(pre[1], C, dev, "pre beta")
+    xt = y.dtype if x is None else x.dtype
+    h, z = (None, None) if out is None else out
+    if h is None:
+        h = torch.empty(y.shape, dtype=xt, device=dev)
+        d.ldh = C
+    else:
+        if h.shape != y.shape or h.dtype != xt or h.device != dev:
+            raise ValueError(f"h must be {xt} {tuple(y.shape)} on {dev}")
+        d.ldh = _row_stride(h, "h")
+    if pre is None:
+        if z is not None:
+            raise ValueError("an output for z without the norm before the next block")
+    elif z is None:
+        z = torch.empty(y.shape, dtype=y.dtype, device=dev)
+        d.ldz = C
+    else:
+        if z.shape != y.shape or z.dtype != y.dtype or z.device != dev:
+            raise ValueError(f"z must be {y.dtype} {tuple(y.shape)} on {dev}")
+        d.ldz = _row_stride(z, "z")
+    if out is not None:
+        for o, ld, own in ((h, d.ldh, x), (z, d.ldz, y)):
+            if o is not None:
+                for t, ldt in ((y, d.ldy), (x, d.ldx), (gate, d.ldgate)):
+                    _refuse_overlap(o, ld, t, ldt, "an output and an input", t is own)
+        _refuse_overlap(h, d.ldh, z, d.ldz, "h and z", False)
+    stats = torch.empty((4, rows), dtype=torch.float32, device=dev) if want_stats else None
+    with on_device(y):
+        check(lib().pe_rnorm_fwd(ctypes.addressof(d), y.data_ptr(), _ptr(x), gp, bp,
+                                 _channel_vector(scale, C, dev, "scale"), _ptr(gate), gq, bq,
+                                 h.data_ptr(), _ptr(z), _ptr(stats), _stream(y)))
+    return h, z, stats
+
+
+def residual_norm_bwd(dh: Optional[torch.Tensor], dz: Optional[torch.Tensor], y: torch.Tensor,
+                      x: Optional[torch.Tensor], stats: Optional[torch.Tensor], *,
+                      norm: str = "layer", post=None, pre=None,
+                      scale: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                      gate_act: str = "none", into: Optional[dict] = None,
+                      workspace: Optional[torch.Tensor] = None) -> dict:
+    """Gradients of residual_norm, called with forward's y, x, stats and options: from dh (h's
+    type, or None for 0) and dz (y's type, given exactly when `pre` is) to a dict of
+
+        dy, dx, dgate (None without x / gate), and float32 [C] dscale, dpost_gamma, dpost_beta,
+        dpre_gamma, dpre_beta (None for a parameter that is None).
+
+    into: tensors of the float32 [C] gradients by name (views of a gradient arena, say), which
+    are overwritten.  x and y must hold what forward read: not after h = x or z = y in place."""
+    d = _block_norm_desc(y, x, gate, gate_act, norm, post, pre, 1.0)
+    C, rows, dev = d.C, d.rows, y.device
+    xt = y.dtype if x is None else x.dtype
+    _need_gpu(dh, dz, stats)
+    if dh is None and dz is None:
+        raise ValueError("neither dh nor dz")
+    if (dz is None) != (pre is None):
+        raise ValueError("dz is given exactly when there is a norm before the next block")
+    for t, dt, name in ((dh, xt, "dh"), (dz, y.dtype, "dz")):
+        if t is not None:
+            if t.shape != y.shape or t.dtype != dt or t.device != dev:
+                raise ValueError(f"{name} must be {dt} {tuple(y.shape)} on {dev}")
+            setattr(d, "ld" + name, _row_stride(t, name))
+    if (post is not None or pre is not None) and (
+            stats is None or stats.dtype != torch.float32 or tuple(stats.shape) != (4, rows)
+            or not stats.is_contiguous() or stats.device != dev):
+        raise ValueError(f"stats must be forward's: contiguous float32 [4, {rows}] on {dev}")
+    given = {"dscale": scale, "dpost_gamma": None, "dpost_beta": None, "dpre_gamma": None,
+             "dpre_beta": None}
+    if post is not None:
+        given["dpost_gamma"], given["dpost_beta"] = post
+    if pre is not None:
+        given["dpre_gamma"], given["dpre_beta"] = pre
+    vec = {k: _channel_vector(t, C, dev, k[1:]) for k, t in given.items()}
+    res = {"dy": torch.empty(y.shape, dtype=y.dtype, device=dev),
+           "dx": None if x is None else torch.empty(y.shape, dtype=xt, device=dev),
+           "dgate": None if gate is None else torch.empty(gate.shape, dtype=y.dtype, device=dev)}
+    d.lddy = d.lddx = d.lddgate = C
+    into = {} if into is None else into
+    unknown = [k for k in into if given.get(k) is None]
+    if unknown:
+        raise ValueError(f"no such parameter gradients: {unknown}")
+    seen = set()
+    for k, t in given.items():
+        o = into.get(k)
+        if o is None:
+            o = None if t is None else torch.empty(C, dtype=torch.float32, device=dev)
+        else:
+            p = _channel_vector(o, C, dev, k)
+            if p in seen:
+                raise ValueError("two parameter gradients share memory")
+            seen.add(p)
+        res[k] = o
+    need = lib().pe_rnorm_bwd_workspace_bytes(ctypes.addressof(d))
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {dev}")
+    if gate is not None and rows == 0:
+        res["dgate"].zero_()
+    with on_device(y):
+        check(lib().pe_rnorm_bwd(
+            ctypes.addressof(d), _ptr(dh), _ptr(dz), y.data_ptr(), _ptr(x), _ptr(stats),
+            vec["dpost_gamma"], vec["dpost_beta"], vec["dscale"], _ptr(gate), vec["dpre_gamma"],
+            res["dy"].data_ptr(), _ptr(res["dx"]), _ptr(res["dgate"]), _ptr(res["dpost_gamma"]),
+            _ptr(res["dpost_beta"]), _ptr(res["dscale"]), _ptr(res["dpre_gamma"]),
+            _ptr(res["dpre_beta"]), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _stream(y)))
+    return res

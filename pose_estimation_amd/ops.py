@@ -3,14 +3,16 @@ and for the current HIP stream; all arithmetic happens in libpe_hip.so.
 """
 from __future__ import annotations
 
+import ctypes
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
 from . import _ffi
-from ._ffi import PE_DTYPE_BF16, PE_DTYPE_F32, check, lib
+from ._ffi import (PE_DTYPE_BF16, PE_DTYPE_F32, PE_NORM_INF, PE_NORM_L2, PE_NORM_MAX_BLOCKS,
+                   ClipDesc, check, lib)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -322,11 +324,34 @@ def adam_scalars(lr: float, beta1: float, beta2: float, step: int, tf1: bool = T
     return lr / bc1, 1.0 / math.sqrt(bc2)
 
 
+def _clip_desc(max_norm: float, norm_type: float, grad_scale: float, skip_nonfinite: bool,
+               norm_over: Optional["GradSet"], like: torch.Tensor) -> ClipDesc:
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
+    if norm_over is None:
+        return ClipDesc(None, None, max_norm, -1, _norm_kind(norm_type), grad_scale,
+                        int(bool(skip_nonfinite)))
+    if norm_over.device != like.device:
+        raise ValueError(f"norm_over is on {norm_over.device}, the parameters on {like.device}")
+    spans, begin, blocks = norm_over._on_stream()
+    return ClipDesc(spans, begin, max_norm, blocks, _norm_kind(norm_type), grad_scale,
+                    int(bool(skip_nonfinite)))
+
+
 def adam_step(p: torch.Tensor, m: torch.Tensor, v: torch.Tensor, grad: torch.Tensor,
               step: int, lr: float = 1e-3, beta1: float = 0.9, beta2: float = 0.999,
               eps: float = 1e-8, p_bf16: Optional[torch.Tensor] = None, tf1: bool = True,
-              grad_scale: float = 1.0) -> None:
-    """In-place Adam over flat float32 arenas (p, m, v updated; p_bf16 receives the copy)."""
+              grad_scale: float = 1.0, max_norm: Optional[float] = None, norm_type: float = 2.0,
+              skip_nonfinite: bool = False, norm_over: Optional["GradSet"] = None,
+              workspace: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """In-place Adam over flat float32 arenas (p, m, v updated; p_bf16 receives the copy).
+
+    max_norm: clip the gradients (times grad_scale) to this global norm inside the step, which
+    leaves `grad` as it is, and return the norm before clipping, [1] float32 on the device.
+    The norm is taken over `grad`, or over `norm_over`, a GradSet, where the arena is only a
+    part of what is clipped together.  A norm that is not finite makes every parameter NaN, or
+    with skip_nonfinite leaves p, m, v and p_bf16 untouched; max_norm = inf only skips."""
     _need_gpu(p, m, v, grad, p_bf16)
     for t in (p, m, v, grad):
         if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != p.numel():
@@ -335,20 +360,228 @@ def adam_step(p: torch.Tensor, m: torch.Tensor, v: torch.Tensor, grad: torch.Ten
                                or not p_bf16.is_contiguous()):
         raise ValueError("p_bf16 must be contiguous bfloat16 of the same length")
     s, a = adam_scalars(lr, beta1, beta2, step, tf1)
+    if max_norm is not None:
+        d = _clip_desc(max_norm, norm_type, grad_scale, skip_nonfinite, norm_over, p)
+        norm, workspace = _norm_buffers(p.device, None, workspace)
+        with on_device(p):
+            check(lib().pe_adam_clip_step(p.data_ptr(), m.data_ptr(), v.data_ptr(),
+                                          grad.data_ptr(), _ptr(p_bf16), p.numel(), beta1, beta2,
+                                          eps, s, a, ctypes.addressof(d), norm.data_ptr(),
+                                          workspace.data_ptr(), _stream(p)))
+        return norm
+    _no_clip(skip_nonfinite, norm_over)
     with on_device(p):
         check(lib().pe_adam_step(p.data_ptr(), m.data_ptr(), v.data_ptr(), grad.data_ptr(),
                                  _ptr(p_bf16), p.numel(), beta1, beta2, eps, s, a, grad_scale,
                                  _stream(p)))
+    return None
+
+
+def _no_clip(skip_nonfinite: bool, norm_over) -> None:
+    if skip_nonfinite or norm_over is not None:
+        raise ValueError("skip_nonfinite and norm_over need max_norm (inf: no clipping)")
 
 
 def sgd_step(p: torch.Tensor, mom: torch.Tensor, grad: torch.Tensor, lr: float,
              momentum: float = 0.9, p_bf16: Optional[torch.Tensor] = None,
-             grad_scale: float = 1.0) -> None:
-    """In-place momentum SGD over flat float32 arenas."""
+             grad_scale: float = 1.0, max_norm: Optional[float] = None, norm_type: float = 2.0,
+             skip_nonfinite: bool = False, norm_over: Optional["GradSet"] = None,
+             workspace: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """In-place momentum SGD over flat float32 arenas; clipping as in adam_step."""
     _need_gpu(p, mom, grad, p_bf16)
     for t in (p, mom, grad):
         if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != p.numel():
             raise ValueError("sgd arenas must be contiguous float32 of equal length")
+    if max_norm is not None:
+        if p_bf16 is not None and (p_bf16.dtype != torch.bfloat16 or not p_bf16.is_contiguous()
+                                   or p_bf16.numel() != p.numel()):
+            raise ValueError("p_bf16 must be contiguous bfloat16 of the same length")
+        d = _clip_desc(max_norm, norm_type, grad_scale, skip_nonfinite, norm_over, p)
+        norm, workspace = _norm_buffers(p.device, None, workspace)
+        with on_device(p):
+            check(lib().pe_sgd_clip_step(p.data_ptr(), mom.data_ptr(), grad.data_ptr(),
+                                         _ptr(p_bf16), p.numel(), lr, momentum,
+                                         ctypes.addressof(d), norm.data_ptr(),
+                                         workspace.data_ptr(), _stream(p)))
+        return norm
+    _no_clip(skip_nonfinite, norm_over)
     with on_device(p):
         check(lib().pe_sgd_step(p.data_ptr(), mom.data_ptr(), grad.data_ptr(), _ptr(p_bf16),
                                 p.numel(), lr, momentum, grad_scale, _stream(p)))
+    return None
+
+
+# ---------------------------------------------------------------------------
+# a8 global gradient norm, clipping
+# ---------------------------------------------------------------------------
+def _norm_kind(norm_type: float) -> int:
+    if norm_type == 2:
+        return PE_NORM_L2
+    if norm_type == math.inf:
+        return PE_NORM_INF
+    raise ValueError(f"norm_type must be 2 or inf, got {norm_type!r}")
+
+
+def _norm_buffers(device, out: Optional[torch.Tensor], workspace: Optional[torch.Tensor]):
+    if out is None:
+        out = torch.empty(1, dtype=torch.float32, device=device)
+    elif out.device != device or out.dtype != torch.float32 or out.numel() != 1:
+        raise ValueError(f"the norm goes to one float32 element on {device}")
+    if workspace is None:
+        workspace = torch.empty(_NORM_WS, dtype=torch.uint8, device=device)
+    elif workspace.device != device or not workspace.is_contiguous() or \
+            workspace.numel() * workspace.element_size() < _NORM_WS:
+        raise ValueError(f"workspace must be contiguous, {_NORM_WS} bytes on {device}")
+    return out, workspace
+
+
+_NORM_WS = 8 * PE_NORM_MAX_BLOCKS
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill one range of memory, each once, in any order of dimensions."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+class GradSet:
+    """A fixed list of gradient tensors (float32 or bfloat16, of any sizes and in any dense
+    layout, empty ones among them) that grad_norm, clip_grads and the clipped optimizer steps
+    take as one.  `out`: where clip_grads writes, one tensor per gradient, of its type, shape and
+    strides (the gradient itself allowed); None: in place.
+
+    The set keeps the tensors and reads their values anew at every call, so a program builds it
+    once over the gradients that every step refills in place.  Tensors that share memory with
+    one another are refused: they would count twice, and be scaled twice."""
+
+    _SPAN = np.dtype([("src", np.uint64), ("dst", np.uint64), ("n", np.int64),
+                      ("dtype", np.int32), ("reserved", np.int32)])
+    # A workgroup's share, at least: below it a launch of fewer, busier workgroups is as fast.
+    MIN_SHARE = 16384
+
+    def __init__(self, tensors: Sequence[torch.Tensor],
+                 out: Optional[Sequence[torch.Tensor]] = None):
+        self.tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+        if not self.tensors:
+            raise ValueError("a GradSet needs at least one tensor")
+        self.out = self.tensors if out is None else (
+            [out] if isinstance(out, torch.Tensor) else list(out))
+        if len(self.out) != len(self.tensors):
+            raise ValueError(f"{len(self.out)} outputs for {len(self.tensors)} gradients")
+        _need_gpu(*self.tensors, *self.out)
+        self.device = self.tensors[0].device
+        self.numel = 0
+        spans, ranges = [], []
+        for t, o in zip(self.tensors, self.out):
+            if t.device != self.device or o.device != self.device:
+                raise ValueError("the tensors of a GradSet are on one device")
+            if t.dtype not in (torch.float32, torch.bfloat16):
+                raise ValueError(f"gradients must be float32 or bfloat16, got {t.dtype}")
+            if o.dtype != t.dtype or o.shape != t.shape or \
+                    (o.stride() != t.stride() and not (t.is_contiguous() and o.is_contiguous())):
+                raise ValueError("an output has its gradient's type, shape and strides")
+            if not _dense(t):
+                raise ValueError(f"gradients must fill their memory: shape {tuple(t.shape)}, "
+                                 f"strides {t.stride()}")
+            n, size = t.numel(), t.element_size()
+            if n == 0:
+                continue
+            self.numel += n
+            src, dst = t.data_ptr(), o.data_ptr()
+            spans.append((src, dst, n, size))
+            ranges.append((src, src + n * size))
+            if dst != src:
+                ranges.append((dst, dst + n * size))
+        ranges.sort()
+        if any(a[1] > b[0] for a, b in zip(ranges, ranges[1:])):
+            raise ValueError("tensors of a GradSet share memory")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("build the GradSet before the capture: its table is copied from "
+                               "the host")
+        with torch.cuda.device(self.device):
+            self._table, self.blocks = self._cut(spans)
+            self._stream = _stream(self._table)
+        self._begin = self._table.data_ptr() + self._spans * self._SPAN.itemsize
+
+    def _cut(self, spans):
+        """One contiguous share of the bytes per workgroup, cut at 16-byte steps of a tensor."""
+        total = sum(n * size for _, _, n, size in spans)
+        share = max(self.MIN_SHARE, -(-total // PE_NORM_MAX_BLOCKS))
+        rows, begin, filled = [], [0], 0
+        for src, dst, n, size in spans:
+            at, left = 0, n * size
+            while left:
+                take = min(left, (share - filled + 15) // 16 * 16)
+                rows.append((src + at, dst + at, take // size,
+                             PE_DTYPE_F32 if size == 4 else PE_DTYPE_BF16, 0))
+                at, left, filled = at + take, left - take, filled + take
+                if filled >= share:
+                    begin.append(len(rows))
+                    filled = 0
+        if filled:
+            begin.append(len(rows))
+        self._spans = len(rows)
+        packed = np.array(rows, dtype=self._SPAN).tobytes() + np.array(begin, np.int32).tobytes()
+        table = torch.from_numpy(np.frombuffer(packed, np.uint8).copy()).to(self.device)
+        return table, len(begin) - 1
+
+    def _on_stream(self):
+        """(spans, begin, blocks) for a launch on the device's current stream.  The allocator is
+        told of a stream other than the set's own; a captured graph keeps the addresses, so the
+        set has to outlive it."""
+        if _stream(self._table) != self._stream and \
+                not torch.cuda.is_current_stream_capturing():
+            self._table.record_stream(torch.cuda.current_stream(self.device))
+        return self._table.data_ptr(), self._begin, self.blocks
+
+    def __len__(self) -> int:
+        return len(self.tensors)
+
+
+def _as_set(grads) -> GradSet:
+    return grads if isinstance(grads, GradSet) else GradSet(grads)
+
+
+def grad_norm(grads, norm_type: float = 2.0, grad_scale: float = 1.0,
+              out: Optional[torch.Tensor] = None,
+              workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Global norm of grad_scale * every gradient -> [1] float32 on the device (no host sync).
+
+    grads: a GradSet, or a tensor or sequence of tensors, for which a set is made for this call.
+    norm_type: 2 (squares summed in float64) or inf (the largest magnitude).  NaN and infinities
+    carry over to the norm."""
+    s = _as_set(grads)
+    kind = _norm_kind(norm_type)
+    out, workspace = _norm_buffers(s.device, out, workspace)
+    with on_device(out):
+        spans, begin, blocks = s._on_stream()
+        check(lib().pe_grad_norm(spans, begin, blocks, kind, grad_scale, out.data_ptr(),
+                                 workspace.data_ptr(), _stream(out)))
+    return out
+
+
+def clip_grads(grads, max_norm: float, norm_type: float = 2.0, grad_scale: float = 1.0,
+               out: Optional[torch.Tensor] = None,
+               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """g * grad_scale * min(1, max_norm / norm) for every gradient of the set, in place or into
+    the set's `out`, rounded once; norm = grad_norm(grads, norm_type, grad_scale), returned as
+    [1] float32 on the device (in `out` if given).  A norm that is not finite makes every result
+    NaN, as TensorFlow's clip_by_global_norm does, the framework of the reference
+    (test.ipynb:19); there is no epsilon, so a norm within the limit changes no bit."""
+    s = _as_set(grads)
+    kind = _norm_kind(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
+    out, workspace = _norm_buffers(s.device, out, workspace)
+    with on_device(out):
+        spans, begin, blocks = s._on_stream()
+        check(lib().pe_grad_clip(spans, begin, blocks, kind, grad_scale, max_norm, out.data_ptr(),
+                                 workspace.data_ptr(), _stream(out)))
+    return out

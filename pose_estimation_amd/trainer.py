@@ -239,6 +239,12 @@ class Trainer:
             if bb is None:
                 bb = self._bbox_labels(joints, H, W)     # the person box spans every joint
             kw["det_labels"] = (bb["classes"], bb["weights"], bb["regs"])
+        clip = t.get("gradient_clip_norm")
+        if clip is not None:
+            kw["clip_norm"] = float(clip)
+        if t.get("skip_nonfinite_steps"):
+            kw.setdefault("clip_norm", float("inf"))
+            kw["skip_nonfinite"] = True
         joints = self._trained(joints)
         lr = learning_rate_at(t, self.global_step)
         opt = t.optimizer
@@ -257,6 +263,12 @@ class Trainer:
             raise ValueError(f"unknown optimizer {name!r}")
         self.global_step += 1
         return loss
+
+    @property
+    def grad_norm(self) -> Optional[torch.Tensor]:
+        """Global gradient norm of the last step before clipping, [1] on the device (no sync);
+        None unless the configuration asks for clipping or for skipping."""
+        return None if self.net is None else self.net.grad_norm
 
     def predict(self, images_u8: torch.Tensor) -> torch.Tensor:
         """uint8 [B,H,W,3] -> float32 heat maps [B,K,H/4,W/4] (running BN statistics)."""

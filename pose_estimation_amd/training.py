@@ -38,6 +38,7 @@ class TrainablePoseResNet(PoseResNet):
         self.opt_m = torch.zeros(self.n_params, dtype=torch.float32, device=dev)
         self.opt_v = torch.zeros(self.n_params, dtype=torch.float32, device=dev)
         self.step_count = 0
+        self.grad_norm: Optional[torch.Tensor] = None   # of the last clipped step
         # transposed weights for the backward-data passes
         self.wt: Dict[str, torch.Tensor] = {}
         for c in self.convs:
@@ -510,10 +511,14 @@ class TrainablePoseResNet(PoseResNet):
                    mask: Optional[torch.Tensor] = None, lr: float = 1e-3, optimizer: str = "adam",
                    beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
                    momentum: float = 0.9, x_s2d: Optional[torch.Tensor] = None,
-                   host_replay: bool = False):
+                   host_replay: bool = False, clip_norm: Optional[float] = None,
+                   skip_nonfinite: bool = False):
         """images uint8 [B,H,W,3] (or None with x_s2d given, see forward_train); joints float32
         [B,K,3] (x, y, v) in input pixels; mask uint8 [B,H/4,W/4] or None.  host_replay: enqueue
         the forward/loss/backward pass from the call list recorded on the first step.
+        clip_norm: limit of the gradients' global norm, taken after the exchange, so that every
+        rank clips alike; self.grad_norm is then the norm before clipping ([1], on the device).
+        skip_nonfinite: leave parameters and moments as they are when that norm is not finite.
         Returns (loss [1] float32 device tensor, per_joint [K])."""
         if host_replay:
             loss, per_joint = self.replay_host(self._pass, images_u8, x_s2d, joints, mask)
@@ -525,11 +530,14 @@ class TrainablePoseResNet(PoseResNet):
             scale = self.bucketer.grad_scale
         self.step_count += 1
         if optimizer == "adam":
-            ops.adam_step(self.master, self.opt_m, self.opt_v, self.grads, self.step_count, lr,
-                          beta1, beta2, eps, p_bf16=self.work, tf1=True, grad_scale=scale)
+            self.grad_norm = ops.adam_step(self.master, self.opt_m, self.opt_v, self.grads,
+                                           self.step_count, lr, beta1, beta2, eps,
+                                           p_bf16=self.work, tf1=True, grad_scale=scale,
+                                           max_norm=clip_norm, skip_nonfinite=skip_nonfinite)
         elif optimizer == "sgd":
-            ops.sgd_step(self.master, self.opt_m, self.grads, lr, momentum, p_bf16=self.work,
-                         grad_scale=scale)
+            self.grad_norm = ops.sgd_step(self.master, self.opt_m, self.grads, lr, momentum,
+                                          p_bf16=self.work, grad_scale=scale, max_norm=clip_norm,
+                                          skip_nonfinite=skip_nonfinite)
         else:
             raise ValueError(f"unknown optimizer {optimizer!r}")
         # the backward-data weights are not needed before the next backward pass: their re-pack
