@@ -45,6 +45,8 @@ struct RnBwd {
 };
 
 // ---- a thread's eight channels ------------------------------------------------------------
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
 template <int TEAM>
 __device__ __forceinline__ int team_size() {
     return TEAM ? TEAM : (int)blockDim.x;
@@ -57,55 +59,47 @@ __device__ __forceinline__ int channel(int t, int T, int j) {
     return VEC ? t * kRnEl + j : t + j * T;
 }
 
+__device__ __forceinline__ f32x8 splat(float v) { return f32x8{v, v, v, v, v, v, v, v}; }
+
+// Channels past C read as 0.
 template <bool VEC>
-__device__ __forceinline__ void load8(const float* p, int t, int T, int C, float* f) {
+__device__ __forceinline__ f32x8 load8(const float* p, int t, int T, int C) {
+    f32x8 f = splat(0.0f);
     if (VEC) {
         if (t * kRnEl < C) {
             const f32x4 a = *reinterpret_cast<const f32x4*>(p + t * kRnEl);
             const f32x4 b = *reinterpret_cast<const f32x4*>(p + t * kRnEl + 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f[j] = a[j];
-                f[4 + j] = b[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) f[j] = 0.0f;
+            f = f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < kRnEl; ++j) {
-            const int c = t + j * T;
-            f[j] = c < C ? p[c] : 0.0f;
-        }
+        for (int j = 0; j < kRnEl; ++j)
+            if (t + j * T < C) f[j] = p[t + j * T];
     }
+    return f;
 }
 
 template <bool VEC>
-__device__ __forceinline__ void load8(const uint16_t* p, int t, int T, int C, float* f) {
+__device__ __forceinline__ f32x8 load8(const uint16_t* p, int t, int T, int C) {
+    f32x8 f = splat(0.0f);
     if (VEC) {
-        if (t * kRnEl < C) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(p + t * kRnEl);
+        u32x4 v = {0, 0, 0, 0};
+        if (t * kRnEl < C) v = *reinterpret_cast<const u32x4*>(p + t * kRnEl);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f[2 * j] = bf16_bits_to_float(v[j] & 0xffffu);
-                f[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) f[j] = 0.0f;
+        for (int j = 0; j < 4; ++j) {
+            f[2 * j] = bf16_bits_to_float(v[j] & 0xffffu);
+            f[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < kRnEl; ++j) {
-            const int c = t + j * T;
-            f[j] = c < C ? bf16_bits_to_float(p[c]) : 0.0f;
-        }
+        for (int j = 0; j < kRnEl; ++j)
+            if (t + j * T < C) f[j] = bf16_bits_to_float(p[t + j * T]);
     }
+    return f;
 }
 
 template <bool VEC>
-__device__ __forceinline__ void store8(float* p, int t, int T, int C, const float* f) {
+__device__ __forceinline__ void store8(float* p, int t, int T, int C, f32x8 f) {
     if (VEC) {
         if (t * kRnEl < C) {
             *reinterpret_cast<f32x4*>(p + t * kRnEl) = f32x4{f[0], f[1], f[2], f[3]};
@@ -113,15 +107,13 @@ __device__ __forceinline__ void store8(float* p, int t, int T, int C, const floa
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < kRnEl; ++j) {
-            const int c = t + j * T;
-            if (c < C) p[c] = f[j];
-        }
+        for (int j = 0; j < kRnEl; ++j)
+            if (t + j * T < C) p[t + j * T] = f[j];
     }
 }
 
 template <bool VEC>
-__device__ __forceinline__ void store8(uint16_t* p, int t, int T, int C, const float* f) {
+__device__ __forceinline__ void store8(uint16_t* p, int t, int T, int C, f32x8 f) {
     if (VEC) {
         if (t * kRnEl < C) {
             u32x4 v;
@@ -131,21 +123,31 @@ __device__ __forceinline__ void store8(uint16_t* p, int t, int T, int C, const f
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < kRnEl; ++j) {
-            const int c = t + j * T;
-            if (c < C) p[c] = (uint16_t)float_to_bf16_bits(f[j]);
-        }
+        for (int j = 0; j < kRnEl; ++j)
+            if (t + j * T < C) p[t + j * T] = (uint16_t)float_to_bf16_bits(f[j]);
     }
 }
 
 template <bool VEC>
-__device__ __forceinline__ void load_param(const float* p, float absent, int t, int T, int C, float* f) {
-    if (p) {
-        load8<VEC>(p, t, T, C, f);
+__device__ __forceinline__ f32x8 load_param(const float* p, float absent, int t, int T, int C) {
+    return p ? load8<VEC>(p, t, T, C) : splat(absent);
+}
+
+__device__ __forceinline__ float sum8(f32x8 v) {
+    return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+}
+
+// 0 in the place of channels past C.
+template <bool VEC>
+__device__ __forceinline__ f32x8 inside(f32x8 v, int t, int T, int C) {
+    if (VEC) {
+        if (t * kRnEl >= C) v = splat(0.0f);
     } else {
 #pragma unroll
-        for (int j = 0; j < kRnEl; ++j) f[j] = absent;
+        for (int j = 0; j < kRnEl; ++j)
+            if (t + j * T >= C) v[j] = 0.0f;
     }
+    return v;
 }
 
 // ---- sums over a row's team ---------------------------------------------------------------
@@ -180,29 +182,23 @@ __device__ __forceinline__ void team_sum2(float& a, float& b, TeamSums& ts) {
     }
 }
 
-// mean and rstd of the row, v replaced by the normalised row.
+// mean and rstd of the row, v replaced by the normalised row (anything past C).
 template <int TEAM, bool VEC>
-__device__ __forceinline__ void normalise(float* v, int t, int T, int C, float inv_c, float eps,
+__device__ __forceinline__ void normalise(f32x8& v, int t, int T, int C, float inv_c, float eps,
                                           bool layer, float& mean, float& rstd, TeamSums& ts) {
     mean = 0.0f;
     float unused = 0.0f;
     if (layer) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kRnEl; ++j) sum += v[j];   // channels past C hold 0
+        float sum = sum8(v);   // channels past C hold 0
         team_sum2<TEAM>(sum, unused, ts);
         mean = sum * inv_c;
+        v -= mean;
     }
-    float sq = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kRnEl; ++j) {
-        v[j] -= mean;
-        if (channel<VEC>(t, T, j) < C) sq += v[j] * v[j];
-    }
+    const f32x8 in = inside<VEC>(v, t, T, C);
+    float sq = sum8(in * in);
     team_sum2<TEAM>(sq, unused, ts);
     rstd = 1.0f / sqrtf(sq * inv_c + eps);
-#pragma unroll
-    for (int j = 0; j < kRnEl; ++j) v[j] *= rstd;
+    v *= rstd;
 }
 
 // ---- gate ---------------------------------------------------------------------------------
@@ -225,6 +221,15 @@ __device__ __forceinline__ float gate_value(float g, int act, float& slope) {
     return g * s;
 }
 
+__device__ __forceinline__ void gate8(f32x8 g, int act, f32x8& phi, f32x8& slope) {
+#pragma unroll
+    for (int j = 0; j < kRnEl; ++j) {
+        float d;
+        phi[j] = gate_value(g[j], act, d);
+        slope[j] = d;
+    }
+}
+
 __device__ __forceinline__ long gate_row(long row, long per) {
     if (per == 1) return row;
     if (row <= 0x7fffffffl && per <= 0x7fffffffl) return (long)((unsigned)row / (unsigned)per);
@@ -240,40 +245,24 @@ __global__ __launch_bounds__(TEAM ? kRnThreads : 1024) void rnorm_fwd_kernel(RnF
     const int t = TEAM ? (int)threadIdx.x % T : (int)threadIdx.x;
     const int teams = TEAM ? kRnThreads / T : 1;
     const int C = a.C;
-    float A[kRnEl], B[kRnEl], gq[kRnEl], bq[kRnEl], phi[kRnEl];
-    {
-        float s[kRnEl];
-        load_param<VEC>(a.gp, 1.0f, t, T, C, A);
-        load_param<VEC>(a.bp, 0.0f, t, T, C, B);
-        load_param<VEC>(a.s, 1.0f, t, T, C, s);
-#pragma unroll
-        for (int j = 0; j < kRnEl; ++j) {
-            A[j] *= s[j];
-            B[j] *= s[j];
-            phi[j] = 1.0f;
-        }
-    }
-    load_param<VEC>(a.gq, 1.0f, t, T, C, gq);
-    load_param<VEC>(a.bq, 0.0f, t, T, C, bq);
+    const f32x8 s = load_param<VEC>(a.s, 1.0f, t, T, C);
+    const f32x8 A = load_param<VEC>(a.gp, 1.0f, t, T, C) * s;
+    const f32x8 B = load_param<VEC>(a.bp, 0.0f, t, T, C) * s;
+    const f32x8 gq = load_param<VEC>(a.gq, 1.0f, t, T, C);
+    const f32x8 bq = load_param<VEC>(a.bq, 0.0f, t, T, C);
+    f32x8 phi = splat(1.0f), slope;
     const long lo = (long)blockIdx.x * a.rows_blk;
     const long hi = lo + a.rows_blk < a.rows ? lo + a.rows_blk : a.rows;
     long have = -1;   // the gate row phi holds
     for (long row = lo + (TEAM ? (int)threadIdx.x / T : 0); row < hi; row += teams) {
-        float y[kRnEl], h[kRnEl];
-        load8<VEC>(static_cast<const YT*>(a.y) + row * a.ldy, t, T, C, y);
-        if (a.x) {
-            load8<VEC>(static_cast<const XT*>(a.x) + row * a.ldx, t, T, C, h);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) h[j] = 0.0f;
-        }
+        f32x8 y = load8<VEC>(static_cast<const YT*>(a.y) + row * a.ldy, t, T, C);
+        f32x8 h = splat(0.0f);
+        if (a.x) h = load8<VEC>(static_cast<const XT*>(a.x) + row * a.ldx, t, T, C);
         if (a.gate_rows) {
             const long g = gate_row(row, a.gate_rows);
             if (g != have) {
-                float slope;
-                load8<VEC>(static_cast<const YT*>(a.gate) + g * a.ldg, t, T, C, phi);
-#pragma unroll
-                for (int j = 0; j < kRnEl; ++j) phi[j] = gate_value(phi[j], a.act, slope);
+                gate8(load8<VEC>(static_cast<const YT*>(a.gate) + g * a.ldg, t, T, C), a.act, phi,
+                      slope);
                 have = g;
             }
         }
@@ -285,21 +274,16 @@ __global__ __launch_bounds__(TEAM ? kRnThreads : 1024) void rnorm_fwd_kernel(RnF
                 a.stats[a.rows + row] = rstd;
             }
         }
-#pragma unroll
-        for (int j = 0; j < kRnEl; ++j) h[j] += (y[j] * A[j] + B[j]) * phi[j];
+        h += (y * A + B) * phi;
         store8<VEC>(static_cast<XT*>(a.h) + row * a.ldh, t, T, C, h);
         if (a.pre) {
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j)
-                if (channel<VEC>(t, T, j) >= C) h[j] = 0.0f;
+            h = inside<VEC>(h, t, T, C);
             normalise<TEAM, VEC>(h, t, T, C, a.inv_c, a.eps, a.layer, mean, rstd, ts);
             if (a.stats && t == 0) {
                 if (a.layer) a.stats[2 * a.rows + row] = mean;
                 a.stats[3 * a.rows + row] = rstd;
             }
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) h[j] = h[j] * gq[j] + bq[j];
-            store8<VEC>(static_cast<YT*>(a.z) + row * a.ldz, t, T, C, h);
+            store8<VEC>(static_cast<YT*>(a.z) + row * a.ldz, t, T, C, h * gq + bq);
         }
     }
 }
@@ -324,107 +308,61 @@ __global__ __launch_bounds__(TEAM ? kRnThreads : 1024) void rnorm_bwd_kernel(RnB
     const int t = TEAM ? (int)threadIdx.x % T : (int)threadIdx.x;
     const int teams = TEAM ? kRnThreads / T : 1;
     const int C = a.C;
-    float A[kRnEl], B[kRnEl], gq[kRnEl], phi[kRnEl];
-    {
-        float s[kRnEl];
-        load_param<VEC>(a.gp, 1.0f, t, T, C, A);
-        load_param<VEC>(a.bp, 0.0f, t, T, C, B);
-        load_param<VEC>(a.s, 1.0f, t, T, C, s);
-#pragma unroll
-        for (int j = 0; j < kRnEl; ++j) {
-            A[j] *= s[j];
-            B[j] *= s[j];
-            phi[j] = 1.0f;
-        }
-    }
-    load_param<VEC>(a.gq, 1.0f, t, T, C, gq);
+    const f32x8 s = load_param<VEC>(a.s, 1.0f, t, T, C);
+    const f32x8 A = load_param<VEC>(a.gp, 1.0f, t, T, C) * s;
+    const f32x8 B = load_param<VEC>(a.bp, 0.0f, t, T, C) * s;
+    const f32x8 gq = load_param<VEC>(a.gq, 1.0f, t, T, C);
+    f32x8 phi = splat(1.0f), slope = splat(1.0f);
     const long g = (long)blockIdx.x / a.nseg;
     const long lo = g * a.group + ((long)blockIdx.x - g * a.nseg) * a.rows_blk;
     const long end = (g + 1) * a.group;
     const long hi = lo + a.rows_blk < end ? lo + a.rows_blk : end;
     const bool own_gate = a.gate_rows == 1;
-    if (a.gate_rows > 1) {
-        float slope;
-        load8<VEC>(static_cast<const YT*>(a.gate) + g * a.ldg, t, T, C, phi);
-#pragma unroll
-        for (int j = 0; j < kRnEl; ++j) phi[j] = gate_value(phi[j], a.act, slope);
-    }
-    float q1[kRnEl], q0[kRnEl], p1[kRnEl], p0[kRnEl];
-#pragma unroll
-    for (int j = 0; j < kRnEl; ++j) q1[j] = q0[j] = p1[j] = p0[j] = 0.0f;
+    if (a.gate_rows > 1)
+        gate8(load8<VEC>(static_cast<const YT*>(a.gate) + g * a.ldg, t, T, C), a.act, phi, slope);
+    f32x8 q1 = splat(0.0f), q0 = q1, p1 = q1, p0 = q1;
     for (long row = lo + (TEAM ? (int)threadIdx.x / T : 0); row < hi; row += teams) {
-        float y[kRnEl], x[kRnEl], d[kRnEl], w[kRnEl], slope[kRnEl];
-        load8<VEC>(static_cast<const YT*>(a.y) + row * a.ldy, t, T, C, y);
-        if (a.pre && a.x) {
-            load8<VEC>(static_cast<const XT*>(a.x) + row * a.ldx, t, T, C, x);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) x[j] = 0.0f;
-        }
-        if (a.dh) {
-            load8<VEC>(static_cast<const XT*>(a.dh) + row * a.lddh, t, T, C, d);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) d[j] = 0.0f;
-        }
-        if (own_gate) {
-            load8<VEC>(static_cast<const YT*>(a.gate) + row * a.ldg, t, T, C, phi);
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) phi[j] = gate_value(phi[j], a.act, slope[j]);
-        }
+        f32x8 y = load8<VEC>(static_cast<const YT*>(a.y) + row * a.ldy, t, T, C);
+        f32x8 x = splat(0.0f), d = x, w = x;
+        if (a.pre && a.x) x = load8<VEC>(static_cast<const XT*>(a.x) + row * a.ldx, t, T, C);
+        if (a.dh) d = load8<VEC>(static_cast<const XT*>(a.dh) + row * a.lddh, t, T, C);
+        if (a.pre) w = load8<VEC>(static_cast<const YT*>(a.dz) + row * a.lddz, t, T, C);
+        if (own_gate)
+            gate8(load8<VEC>(static_cast<const YT*>(a.gate) + row * a.ldg, t, T, C), a.act, phi, slope);
         float rp = 1.0f;
         if (a.post) {
             rp = a.stats[a.rows + row];
             const float mean = a.layer ? a.stats[row] : 0.0f;
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) y[j] = (y[j] - mean) * rp;
+            y = (y - mean) * rp;
         }
         if (a.pre) {
             const float rq = a.stats[3 * a.rows + row];
             const float mean = a.layer ? a.stats[2 * a.rows + row] : 0.0f;
-            load8<VEC>(static_cast<const YT*>(a.dz) + row * a.lddz, t, T, C, w);
-            float m1 = 0.0f, m2 = 0.0f;
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) {
-                const float h = x[j] + (y[j] * A[j] + B[j]) * phi[j];
-                const float hhat = (h - mean) * rq;
-                q0[j] += w[j];
-                q1[j] += w[j] * hhat;
-                w[j] *= gq[j];
-                x[j] = hhat;
-                m1 += w[j];
-                m2 += w[j] * hhat;
-            }
+            const f32x8 hhat = (x + (y * A + B) * phi - mean) * rq;
+            q0 += w;
+            q1 += w * hhat;
+            w *= gq;
+            float m1 = sum8(w), m2 = sum8(w * hhat);
             team_sum2<TEAM>(m1, m2, ts);
             m1 = a.layer ? m1 * a.inv_c : 0.0f;
             m2 *= a.inv_c;
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) d[j] += rq * (w[j] - m1 - x[j] * m2);
+            d += (w - m1 - hhat * m2) * rq;
         }
         if (a.dx) store8<VEC>(static_cast<XT*>(a.dx) + row * a.lddx, t, T, C, d);
-        if (own_gate) {
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) w[j] = d[j] * (y[j] * A[j] + B[j]) * slope[j];
-            store8<VEC>(static_cast<YT*>(a.dgate) + row * a.lddg, t, T, C, w);
-        }
-        float n1 = 0.0f, n2 = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kRnEl; ++j) {
-            if (channel<VEC>(t, T, j) >= C) d[j] = 0.0f;
-            const float u = d[j] * phi[j];
-            const float keep = own_gate ? u : d[j];
-            p0[j] += keep;
-            p1[j] += keep * y[j];
-            w[j] = u * A[j];
-            n1 += w[j];
-            n2 += w[j] * y[j];
-        }
+        if (own_gate)
+            store8<VEC>(static_cast<YT*>(a.dgate) + row * a.lddg, t, T, C, d * (y * A + B) * slope);
+        d = inside<VEC>(d, t, T, C);
+        const f32x8 u = d * phi;
+        const f32x8 keep = own_gate ? u : d;
+        p0 += keep;
+        p1 += keep * y;
+        w = u * A;
         if (a.post) {
+            float n1 = sum8(w), n2 = sum8(w * y);
             team_sum2<TEAM>(n1, n2, ts);
             n1 = a.layer ? n1 * a.inv_c : 0.0f;
             n2 *= a.inv_c;
-#pragma unroll
-            for (int j = 0; j < kRnEl; ++j) w[j] = rp * (w[j] - n1 - y[j] * n2);
+            w = (w - n1 - y * n2) * rp;
         }
         store8<VEC>(static_cast<YT*>(a.dy) + row * a.lddy, t, T, C, w);
     }
@@ -432,12 +370,12 @@ __global__ __launch_bounds__(TEAM ? kRnThreads : 1024) void rnorm_bwd_kernel(RnB
     float* out = a.part + (long)blockIdx.x * 4 * C;
     if (TEAM) {
         // rows side by side in the wave, then the waves in order
-        float* sums[4] = {q1, q0, p1, p0};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
+            const f32x8 sums = k == 0 ? q1 : k == 1 ? q0 : k == 2 ? p1 : p0;
 #pragma unroll
             for (int j = 0; j < kRnEl; ++j) {
-                float v = sums[k][j];
+                float v = sums[j];
 #pragma unroll
                 for (int off = 32; off >= (TEAM ? TEAM : 64); off >>= 1) v += __shfl_xor(v, off, 64);
                 if ((int)(threadIdx.x & 63) < T)
