@@ -333,7 +333,7 @@ def test_c_entries_refuse_bad_descriptions():
             d = desc(rows=rows, C=C, gate_rows=per)
             n = need(ctypes.addressof(d))
             items = max(1100, rows // 2) if per == 2 else 1100
-            assert 16 * C <= n <= 16 * C * items
+            assert 16 * C <= n <= 16 * (C + 3) * items
 
 
 def test_the_expected_values_are_those_of_automatic_differentiation():
