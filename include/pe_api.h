@@ -261,17 +261,17 @@ int32_t pe_sgd_step(float* p, float* mom, const float* grad, uint16_t* p_bf16,
  * is NaN; with skip_nonfinite an optimizer step then changes nothing but *norm.
  * The order of the sums depends on the lengths alone: the same gradients give the same bits.
  *
- * A set of tensors is a DEVICE table of contiguous spans, cut so that workgroup b handles spans
- * [begin[b], begin[b+1]) (begin: DEVICE array of blocks + 1 entries, blocks <= PE_NORM_MAX_BLOCKS,
- * the shares about equal).  A span is 1 to 2^62 elements of one type, aligned to its element.
- * dst is where pe_grad_clip writes (src itself for clipping in place); spans must not overlap
- * otherwise.  The other calls read src only.
+ * A set of tensors is a DEVICE table of contiguous spans, cut into shares: a wave handles spans
+ * [begin[i], begin[i+1]) (begin: DEVICE array of shares + 1 entries, shares <= PE_NORM_MAX_SHARES),
+ * so shares should be about equal.  A span is 1 to 2^30 elements of one type, aligned to its
+ * element.  dst is where pe_grad_clip writes (src itself for clipping in place); spans must not
+ * overlap otherwise.  The other calls read src only.
  *
  * workspace: pe_grad_norm_workspace_bytes(), 8-byte aligned; calls that share one must be ordered.
  * ---------------------------------------------------------------------- */
 #define PE_NORM_L2  0
 #define PE_NORM_INF 1
-#define PE_NORM_MAX_BLOCKS 1024
+#define PE_NORM_MAX_SHARES 4096
 
 typedef struct pe_grad_span {
     const void* src;
@@ -282,21 +282,21 @@ typedef struct pe_grad_span {
 } pe_grad_span;
 
 size_t pe_grad_norm_workspace_bytes(void);
-int32_t pe_grad_norm(const pe_grad_span* spans_device, const int32_t* begin_device, int32_t blocks,
+int32_t pe_grad_norm(const pe_grad_span* spans_device, const int32_t* begin_device, int32_t shares,
                      int32_t kind, float grad_scale, float* norm, void* workspace,
                      pe_stream_t stream);
-int32_t pe_grad_clip(const pe_grad_span* spans_device, const int32_t* begin_device, int32_t blocks,
+int32_t pe_grad_clip(const pe_grad_span* spans_device, const int32_t* begin_device, int32_t shares,
                      int32_t kind, float grad_scale, double max_norm, float* norm, void* workspace,
                      pe_stream_t stream);
 
 /* pe_adam_step / pe_sgd_step with clipped gradients: the norm is taken over the set, or over the
- * step's own arena grad[0..n) when blocks is negative; grad itself is not changed.  Within the
+ * step's own arena grad[0..n) when shares is negative; grad itself is not changed.  Within the
  * limit the results have the bits of the plain step with the same grad_scale. */
 typedef struct pe_clip_desc {
-    const pe_grad_span* spans;   /* DEVICE table, see above; unused when blocks < 0 */
+    const pe_grad_span* spans;   /* DEVICE table, see above; unused when shares < 0 */
     const int32_t* begin;
     double max_norm;
-    int32_t blocks;
+    int32_t shares;
     int32_t kind;
     float grad_scale;
     int32_t skip_nonfinite;

@@ -19,7 +19,7 @@ PE_DTYPE_F32 = 0
 PE_DTYPE_BF16 = 1
 PE_NORM_L2 = 0
 PE_NORM_INF = 1
-PE_NORM_MAX_BLOCKS = 1024
+PE_NORM_MAX_SHARES = 4096
 PE_MAX_RADIUS = 31
 PE_MSE_STATIC_MAX_MAPS = 65536
 
@@ -306,7 +306,7 @@ class ClipDesc(ctypes.Structure):
     """Mirror of pe_clip_desc (include/pe_api.h)."""
 
     _fields_ = [("spans", c_void_p), ("begin", c_void_p), ("max_norm", c_double),
-                ("blocks", c_int32), ("kind", c_int32), ("grad_scale", c_float),
+                ("shares", c_int32), ("kind", c_int32), ("grad_scale", c_float),
                 ("skip_nonfinite", c_int32)]
 
 

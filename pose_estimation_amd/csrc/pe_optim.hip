@@ -110,18 +110,36 @@ __global__ __launch_bounds__(256) void sgd_kernel(float* __restrict__ p, float* 
 // once more for the norm, not twice.  Each workgroup folds the partials for itself; 2048 of them
 // keep that at a thousandth of the traffic.  The factor multiplies in float64 and rounds once, so
 // a step whose norm is within the limit has the bits of the plain step.
+constexpr int64_t kFewGradients = 16384;
+
 struct ClipStep {
     const double* part;
     int parts;
     ClipRule rule;
     int skip_nonfinite;
     float* norm;
+    const float* grad;   // parts < 0: no launch before, the norm is over these few_n gradients
+    int few_n;
     // The gradients' factor; false: the norm is not finite and the step is to be skipped.
     __device__ __forceinline__ bool factor(double& f) const {
-        const double n = norm_fold(part, parts, rule);
+        const double n = parts < 0 ? few() : norm_fold(part, parts, rule);
         if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
         f = clip_factor(n, rule);
         return !(skip_nonfinite && !isfinite(n));
+    }
+    // A small arena's norm by every workgroup for itself: a few KB from L2 instead of a launch.
+    __device__ __forceinline__ double few() const {
+        if (rule.kind == PE_NORM_L2) return few<PE_NORM_L2>();
+        return few<PE_NORM_INF>();
+    }
+    template <int KIND>
+    __device__ __forceinline__ double few() const {
+        NormAcc<KIND> acc;
+        const int share = ((few_n + kNormWaves - 1) / kNormWaves + 3) & ~3;
+        const int lo = ((int)threadIdx.x >> 6) * share;
+        if (lo < few_n)
+            norm_span<KIND>(grad + lo, few_n - lo < share ? few_n - lo : share, (int)threadIdx.x & 63, acc);
+        return norm_of(norm_block<kNormThreads>(acc.value(), KIND), rule);
     }
 };
 
@@ -216,7 +234,7 @@ static unsigned clip_grid(long n) {
     return (unsigned)blocks;
 }
 
-// Checks the clipping arguments and enqueues the norm: over the given set, or (blocks < 0) over
+// Checks the clipping arguments and enqueues the norm: over the given set, or (shares < 0) over
 // the step's own gradient arena.
 static int32_t start_clip(const char* what, const float* grad, int64_t n, const pe_clip_desc* d,
                           float* norm, void* workspace, pe_stream_t stream, ClipStep* c) {
@@ -225,9 +243,9 @@ static int32_t start_clip(const char* what, const float* grad, int64_t n, const 
     PE_REQUIRE(isfinite(d->grad_scale), PE_E_INVALID, "%s: grad_scale must be finite", what);
     PE_REQUIRE(d->kind == PE_NORM_L2 || d->kind == PE_NORM_INF, PE_E_UNSUPPORTED,
                "%s: unknown norm %d", what, d->kind);
-    PE_REQUIRE(d->blocks <= kNormMaxParts, PE_E_INVALID, "%s: %d workgroups, at most %d", what,
-               d->blocks, kNormMaxParts);
-    PE_REQUIRE(d->blocks <= 0 || (d->spans && d->begin), PE_E_INVALID, "%s: NULL table", what);
+    PE_REQUIRE(d->shares <= PE_NORM_MAX_SHARES, PE_E_INVALID, "%s: %d shares, at most %d", what,
+               d->shares, PE_NORM_MAX_SHARES);
+    PE_REQUIRE(d->shares <= 0 || (d->spans && d->begin), PE_E_INVALID, "%s: NULL table", what);
     PE_REQUIRE(norm && workspace, PE_E_INVALID, "%s: NULL norm or workspace", what);
     PE_REQUIRE(aligned(workspace, 8), PE_E_INVALID, "%s: workspace must be 8-byte aligned", what);
     double* part = static_cast<double*>(workspace);
@@ -235,11 +253,15 @@ static int32_t start_clip(const char* what, const float* grad, int64_t n, const 
     c->rule = ClipRule{(double)d->grad_scale, d->max_norm, d->kind};
     c->skip_nonfinite = d->skip_nonfinite;
     c->norm = norm;
-    if (d->blocks >= 0) {
-        c->parts = d->blocks;
-        launch_norm_parts(d->spans, d->begin, d->blocks, d->kind, part, as_stream(stream));
+    c->grad = grad;
+    c->few_n = 0;
+    if (d->shares >= 0) {
+        c->parts = launch_norm_parts(d->spans, d->begin, d->shares, d->kind, part, as_stream(stream));
+    } else if (n <= kFewGradients) {
+        c->parts = -1;
+        c->few_n = (int)n;
     } else {
-        launch_flat_norm(grad, (long)n, d->kind, part, &c->parts, as_stream(stream));
+        c->parts = launch_flat_norm(grad, (long)n, d->kind, part, as_stream(stream));
     }
     return PE_OK;
 }

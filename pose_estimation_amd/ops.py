@@ -11,7 +11,7 @@ import numpy as np
 import torch
 
 from . import _ffi
-from ._ffi import (PE_DTYPE_BF16, PE_DTYPE_F32, PE_NORM_INF, PE_NORM_L2, PE_NORM_MAX_BLOCKS,
+from ._ffi import (PE_DTYPE_BF16, PE_DTYPE_F32, PE_NORM_INF, PE_NORM_L2, PE_NORM_MAX_SHARES,
                    ClipDesc, check, lib)
 
 
@@ -334,8 +334,8 @@ def _clip_desc(max_norm: float, norm_type: float, grad_scale: float, skip_nonfin
                         int(bool(skip_nonfinite)))
     if norm_over.device != like.device:
         raise ValueError(f"norm_over is on {norm_over.device}, the parameters on {like.device}")
-    spans, begin, blocks = norm_over._on_stream()
-    return ClipDesc(spans, begin, max_norm, blocks, _norm_kind(norm_type), grad_scale,
+    spans, begin, shares = norm_over._on_stream()
+    return ClipDesc(spans, begin, max_norm, shares, _norm_kind(norm_type), grad_scale,
                     int(bool(skip_nonfinite)))
 
 
@@ -435,7 +435,7 @@ def _norm_buffers(device, out: Optional[torch.Tensor], workspace: Optional[torch
     return out, workspace
 
 
-_NORM_WS = 8 * PE_NORM_MAX_BLOCKS
+_NORM_WS = 2 * PE_NORM_MAX_SHARES   # a float64 for every four shares
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -462,8 +462,8 @@ class GradSet:
 
     _SPAN = np.dtype([("src", np.uint64), ("dst", np.uint64), ("n", np.int64),
                       ("dtype", np.int32), ("reserved", np.int32)])
-    # A workgroup's share, at least: below it a launch of fewer, busier workgroups is as fast.
-    MIN_SHARE = 16384
+    # Bytes of a wave's share, at least, and what a tensor's start counts beside its bytes.
+    MIN_SHARE, START = 8192, 1024
 
     def __init__(self, tensors: Sequence[torch.Tensor],
                  out: Optional[Sequence[torch.Tensor]] = None):
@@ -505,40 +505,45 @@ class GradSet:
             raise RuntimeError("build the GradSet before the capture: its table is copied from "
                                "the host")
         with torch.cuda.device(self.device):
-            self._table, self.blocks = self._cut(spans)
+            self._table, self.shares = self._cut(spans)
             self._stream = _stream(self._table)
         self._begin = self._table.data_ptr() + self._spans * self._SPAN.itemsize
 
     def _cut(self, spans):
-        """One contiguous share of the bytes per workgroup, cut at 16-byte steps of a tensor."""
-        total = sum(n * size for _, _, n, size in spans)
-        share = max(self.MIN_SHARE, -(-total // PE_NORM_MAX_BLOCKS))
-        rows, begin, filled = [], [0], 0
-        for src, dst, n, size in spans:
-            at, left = 0, n * size
-            while left:
-                take = min(left, (share - filled + 15) // 16 * 16)
-                rows.append((src + at, dst + at, take // size,
-                             PE_DTYPE_F32 if size == 4 else PE_DTYPE_BF16, 0))
-                at, left, filled = at + take, left - take, filled + take
-                if filled >= share:
-                    begin.append(len(rows))
-                    filled = 0
-        if filled:
-            begin.append(len(rows))
+        """(table on the device, number of shares).  The tensors lie end to end on a line, each
+        with START idle bytes behind it; a share is what lies between two of its equal marks, so
+        spans start at 16-byte steps of their tensor."""
+        if not spans:
+            self._spans = 0
+            return torch.zeros(1, dtype=torch.int32, device=self.device), 0
+        src, dst, n, size = (np.array(v, np.int64) for v in zip(*spans))
+        nbytes = n * size
+        room = (nbytes + 15) // 16 * 16 + self.START
+        at = np.cumsum(room) - room
+        share = max(self.MIN_SHARE, (-(-int(room.sum()) // PE_NORM_MAX_SHARES) + 15) // 16 * 16)
+        first, last = at // share, (at + nbytes - 1) // share
+        count = last - first + 1
+        i = np.repeat(np.arange(len(n)), count)              # the tensor of each span
+        k = np.arange(len(i)) - np.repeat(np.cumsum(count) - count, count) + first[i]
+        lo = np.maximum(k * share - at[i], 0)
+        hi = np.minimum((k + 1) * share - at[i], nbytes[i])
+        rows = np.zeros(len(i), self._SPAN)
+        rows["src"], rows["dst"], rows["n"] = src[i] + lo, dst[i] + lo, (hi - lo) // size[i]
+        rows["dtype"] = np.where(size[i] == 4, PE_DTYPE_F32, PE_DTYPE_BF16)
+        shares = int(k[-1]) + 1
+        begin = np.searchsorted(k, np.arange(shares + 1)).astype(np.int32)
         self._spans = len(rows)
-        packed = np.array(rows, dtype=self._SPAN).tobytes() + np.array(begin, np.int32).tobytes()
-        table = torch.from_numpy(np.frombuffer(packed, np.uint8).copy()).to(self.device)
-        return table, len(begin) - 1
+        packed = np.frombuffer(rows.tobytes() + begin.tobytes(), np.uint8).copy()
+        return torch.from_numpy(packed).to(self.device), shares
 
     def _on_stream(self):
-        """(spans, begin, blocks) for a launch on the device's current stream.  The allocator is
+        """(spans, begin, shares) for a launch on the device's current stream.  The allocator is
         told of a stream other than the set's own; a captured graph keeps the addresses, so the
         set has to outlive it."""
         if _stream(self._table) != self._stream and \
                 not torch.cuda.is_current_stream_capturing():
             self._table.record_stream(torch.cuda.current_stream(self.device))
-        return self._table.data_ptr(), self._begin, self.blocks
+        return self._table.data_ptr(), self._begin, self.shares
 
     def __len__(self) -> int:
         return len(self.tensors)
@@ -560,8 +565,8 @@ def grad_norm(grads, norm_type: float = 2.0, grad_scale: float = 1.0,
     kind = _norm_kind(norm_type)
     out, workspace = _norm_buffers(s.device, out, workspace)
     with on_device(out):
-        spans, begin, blocks = s._on_stream()
-        check(lib().pe_grad_norm(spans, begin, blocks, kind, grad_scale, out.data_ptr(),
+        spans, begin, shares = s._on_stream()
+        check(lib().pe_grad_norm(spans, begin, shares, kind, grad_scale, out.data_ptr(),
                                  workspace.data_ptr(), _stream(out)))
     return out
 
@@ -581,7 +586,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, grad_scale: float
         raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
     out, workspace = _norm_buffers(s.device, out, workspace)
     with on_device(out):
-        spans, begin, blocks = s._on_stream()
-        check(lib().pe_grad_clip(spans, begin, blocks, kind, grad_scale, max_norm, out.data_ptr(),
+        spans, begin, shares = s._on_stream()
+        check(lib().pe_grad_clip(spans, begin, shares, kind, grad_scale, max_norm, out.data_ptr(),
                                  workspace.data_ptr(), _stream(out)))
     return out

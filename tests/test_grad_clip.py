@@ -25,10 +25,10 @@ def test_c_entries_refuse_bad_arguments_on_the_host():
     lib = _ffi.lib()
     E, U = _ffi.PE_E_INVALID, _ffi.PE_E_UNSUPPORTED
     one = 16   # stands for a pointer: never followed, every call is refused before a launch
-    assert lib.pe_grad_norm_workspace_bytes() == 8 * _ffi.PE_NORM_MAX_BLOCKS
+    assert lib.pe_grad_norm_workspace_bytes() == 2 * _ffi.PE_NORM_MAX_SHARES
     assert lib.pe_grad_norm(None, None, 1, 0, 1.0, one, one, None) == E
     assert lib.pe_grad_norm(one, one, -1, 0, 1.0, one, one, None) == E
-    assert lib.pe_grad_norm(one, one, 1025, 0, 1.0, one, one, None) == E
+    assert lib.pe_grad_norm(one, one, 4097, 0, 1.0, one, one, None) == E
     assert lib.pe_grad_norm(one, one, 1, 7, 1.0, one, one, None) == U
     assert lib.pe_grad_norm(one, one, 1, 0, INF, one, one, None) == E
     assert lib.pe_grad_norm(one, one, 1, 0, 1.0, None, one, None) == E
@@ -47,7 +47,7 @@ def test_c_entries_refuse_bad_arguments_on_the_host():
     assert adam(p=None) == E and adam(grad=8) == E and adam(desc=None) == E and adam(n=-1) == E
     assert adam(norm=None) == E and adam(ws=None) == E and adam(ws=12) == E
     for field, bad, code in (("kind", 3, U), ("grad_scale", math.nan, E), ("max_norm", -2.0, E),
-                             ("max_norm", math.nan, E), ("blocks", 1, E), ("blocks", 2000, E)):
+                             ("max_norm", math.nan, E), ("shares", 1, E), ("shares", 5000, E)):
         b = _ffi.ClipDesc(None, None, 1.0, -1, 0, 1.0, 0)
         setattr(b, field, bad)
         assert adam(desc=b) == code, field
@@ -77,24 +77,27 @@ def test_a_set_refuses_what_it_cannot_hold(on_cpu):
 
 def test_the_cut_covers_every_element_once_in_equal_shares(on_cpu):
     rng = np.random.default_rng(5)
-    for total in (1, 5, 4097, 300_000, 20_000_003):
-        count = min(total, 37)
-        cuts = np.sort(rng.choice(np.arange(1, total), count - 1, replace=False)) if count > 1 else []
+    for total, most in ((1, 1), (5, 5), (4097, 37), (4097, 4097), (300_000, 37), (20_000_003, 400),
+                        (400_000_001, 3)):
+        count = min(total, most)
+        cuts = np.sort(rng.choice(total - 1, count - 1, replace=False) + 1) if count > 1 else []
         sizes = np.diff(np.concatenate([[0], cuts, [total]])).astype(int).tolist()
-        spans = [(1 << 30, 1 << 40, n, 4 if i % 3 else 2) for i, n in enumerate(sizes)]
+        spans = [((i + 1) << 36, (i + 1) << 44, n, 4 if i % 3 else 2) for i, n in enumerate(sizes)]
         s = object.__new__(ops.GradSet)
         s.device = torch.device("cpu")
-        table, blocks = s._cut(spans)
+        table, shares = s._cut(spans)
         raw = table.numpy().tobytes()
         rows = np.frombuffer(raw[:s._spans * 32], dtype=ops.GradSet._SPAN)
         begin = np.frombuffer(raw[s._spans * 32:], dtype=np.int32)
-        assert len(begin) == blocks + 1 <= 1025 and begin[0] == 0 and begin[-1] == len(rows)
+        assert len(begin) == shares + 1 <= 4097 and begin[0] == 0 and begin[-1] == len(rows)
+        assert (np.diff(begin) >= 0).all()
         assert (rows["n"] > 0).all() and int(rows["n"].sum()) == total
         size = np.where(rows["dtype"] == _ffi.PE_DTYPE_F32, 4, 2)
         nbytes = rows["n"] * size
-        loads = [int(nbytes[b:e].sum()) for b, e in zip(begin, begin[1:])]
-        share = max(ops.GradSet.MIN_SHARE, -(-sum(loads) // 1024))
-        assert max(loads) < share + 16 and all(v >= share for v in loads[:-1])
+        weight = sum(n * e for _, _, n, e in spans) + s.START * count
+        limit = max(s.MIN_SHARE, weight / 4096) + 32
+        for b, e in zip(begin, begin[1:]):   # neither many bytes nor many tensors in one share
+            assert int(nbytes[b:e].sum()) <= limit and (e - b - 2) * s.START <= limit
         k = 0
         for src, dst, n, esize in spans:     # in order, contiguous
             at = 0
