@@ -268,10 +268,14 @@ int32_t pe_sgd_step(float* p, float* mom, const float* grad, uint16_t* p_bf16,
  * overlap otherwise.  The other calls read src only.
  *
  * workspace: pe_grad_norm_workspace_bytes(), 8-byte aligned; calls that share one must be ordered.
+ * A set of at most PE_NORM_FEW_SHARES shares needs none in pe_grad_norm and pe_grad_clip (one
+ * launch by one workgroup), an arena of at most PE_NORM_FEW_ELEMENTS none in the steps.
  * ---------------------------------------------------------------------- */
 #define PE_NORM_L2  0
 #define PE_NORM_INF 1
 #define PE_NORM_MAX_SHARES 4096
+#define PE_NORM_FEW_SHARES 16
+#define PE_NORM_FEW_ELEMENTS 16384
 
 typedef struct pe_grad_span {
     const void* src;

@@ -20,6 +20,8 @@ PE_DTYPE_BF16 = 1
 PE_NORM_L2 = 0
 PE_NORM_INF = 1
 PE_NORM_MAX_SHARES = 4096
+PE_NORM_FEW_SHARES = 16
+PE_NORM_FEW_ELEMENTS = 16384
 PE_MAX_RADIUS = 31
 PE_MSE_STATIC_MAX_MAPS = 65536
 

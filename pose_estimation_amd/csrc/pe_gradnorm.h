@@ -10,7 +10,7 @@ constexpr int kNormThreads = 256;
 constexpr int kNormWaves = kNormThreads / kWave;
 constexpr int kNormMaxParts = PE_NORM_MAX_SHARES / kNormWaves;   // partial results of one norm
 
-constexpr int kNormFewShares = 16;   // a set of so few takes one workgroup and one launch
+constexpr int kNormFewShares = PE_NORM_FEW_SHARES;   // a set of so few takes one workgroup and one launch
 
 // What turns the partial results into a factor for the gradients.
 struct ClipRule {

@@ -69,7 +69,6 @@ __global__ __launch_bounds__(kNormThreads) void norm_final_kernel(const double* 
     if (threadIdx.x == 0) *norm = (float)n;
 }
 
-// One wave over n elements, four loads a lane under way.  src and dst may be the same.
 template <typename T>
 __device__ __forceinline__ T scaled_one(T v, double f);
 template <>
@@ -91,6 +90,10 @@ __device__ __forceinline__ u32x4 scaled_vec(u32x4 v, double f) {
     return v;
 }
 
+// One wave over n elements, four loads a lane under way; from and to may be the same.  The stores
+// are non-temporal: ordinary ones push out the gradients that the norm has just left in the
+// caches (34 M float32 into another array: 75 us against 88, with the Adam step that reads them
+// 256 against 266; in place no difference).
 template <typename T>
 __device__ __forceinline__ void clip_span(const T* from, T* to, int n, int lane, double f) {
     typedef typename Vec16<T>::type V;
@@ -109,7 +112,7 @@ __device__ __forceinline__ void clip_span(const T* from, T* to, int n, int lane,
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) v[u] = q[i + 64 * u];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) o[i + 64 * u] = scaled_vec(v[u], f);
+        for (int u = 0; u < AHEAD; ++u) __builtin_nontemporal_store(scaled_vec(v[u], f), o + i + 64 * u);
     }
     for (; i < nv; i += 64) o[i] = scaled_vec(q[i], f);
     const int tail = h + nv * PER + lane;
@@ -205,7 +208,8 @@ static int32_t check_set(const char* what, const pe_grad_span* spans, const int3
     PE_REQUIRE(kind == PE_NORM_L2 || kind == PE_NORM_INF, PE_E_UNSUPPORTED,
                "%s: unknown norm %d", what, kind);
     PE_REQUIRE(isfinite(grad_scale), PE_E_INVALID, "%s: grad_scale must be finite", what);
-    PE_REQUIRE(norm && workspace, PE_E_INVALID, "%s: NULL norm or workspace", what);
+    PE_REQUIRE(norm, PE_E_INVALID, "%s: NULL norm", what);
+    PE_REQUIRE(workspace || shares <= kNormFewShares, PE_E_INVALID, "%s: NULL workspace", what);
     PE_REQUIRE(aligned(workspace, 8), PE_E_INVALID, "%s: workspace must be 8-byte aligned", what);
     return PE_OK;
 }

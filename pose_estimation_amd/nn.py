@@ -1313,6 +1313,7 @@ def bn_bwd(da: torch.Tensor, a: Optional[torch.Tensor], z: torch.Tensor, gamma, 
 
 # --------------------------------------------------------------------------- row norm of a block
 RNORM_MAX_C = 8192
+_INF = float("inf")
 _RNORM_KIND = {"layer": PE_RNORM_LAYER, "rms": PE_RNORM_RMS}
 _GATE_ACT = {"none": PE_GATE_NONE, "sigmoid": PE_GATE_SIGMOID, "silu": PE_GATE_SILU}
 _RNORM_DTYPE = {torch.float32: PE_DTYPE_F32, torch.bfloat16: PE_DTYPE_BF16}
@@ -1337,12 +1338,12 @@ def _row_stride(t: torch.Tensor, name: str) -> int:
     return shape[-1] if ld is None else ld
 
 
-def _channel_vector(t: Optional[torch.Tensor], C: int, device, name: str):
+def _channel_vector(t: Optional[torch.Tensor], C: int, index: int, name: str):
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != C or not t.is_contiguous() or \
-            t.device != device:
-        raise ValueError(f"{name} must be contiguous float32 [{C}] on {device}")
+    if t.dtype is not torch.float32 or t.dim() != 1 or t.numel() != C or not t.is_contiguous() or \
+            t.get_device() != index:
+        raise ValueError(f"{name} must be contiguous float32 [{C}] on the device of y")
     return t.data_ptr()
 
 
@@ -1359,22 +1360,23 @@ def _block_norm_desc(y, x, gate, gate_act, norm, post, pre, eps) -> RnormDesc:
     if yt is None or xt is None or (yt == PE_DTYPE_F32 and xt != PE_DTYPE_F32):
         raise ValueError("y and x must be bfloat16 or float32, x float32 where y is: got "
                          f"{y.dtype}, {None if x is None else x.dtype}")
-    if norm not in _RNORM_KIND:
+    kind, act = _RNORM_KIND.get(norm), _GATE_ACT.get(gate_act)
+    if kind is None:
         raise ValueError(f"unknown norm {norm!r}")
-    if gate_act not in _GATE_ACT:
+    if act is None:
         raise ValueError(f"unknown gate activation {gate_act!r}")
-    if not 0.0 < eps < float("inf"):
+    if not 0.0 < eps < _INF:
         raise ValueError(f"eps must be positive, got {eps}")
-    d = RnormDesc(rows=rows, C=C, y_dtype=yt, x_dtype=xt, norm=_RNORM_KIND[norm],
-                  post=post is not None, pre=pre is not None, gate_act=_GATE_ACT[gate_act],
-                  eps=eps, ldy=_row_stride(y, "y"))
+    d = RnormDesc(rows=rows, C=C, y_dtype=yt, x_dtype=xt, norm=kind, post=post is not None,
+                  pre=pre is not None, gate_act=act, eps=eps,
+                  ldy=C if y.is_contiguous() else _row_stride(y, "y"))
     if x is not None:
         if x.shape != y.shape or x.device != y.device:
             raise ValueError(f"x must be {tuple(y.shape)} on {y.device}, "
                              f"got {tuple(x.shape)} on {x.device}")
-        d.ldx = _row_stride(x, "x")
+        d.ldx = C if x.is_contiguous() else _row_stride(x, "x")
     if gate is None:
-        if gate_act != "none":
+        if act:
             raise ValueError("gate_act without a gate")
         return d
     if gate.dtype != y.dtype or gate.device != y.device or gate.dim() < 1 or gate.shape[-1] != C:
@@ -1386,6 +1388,12 @@ def _block_norm_desc(y, x, gate, gate_act, norm, post, pre, eps) -> RnormDesc:
     d.gate_rows = rows // G if G else 0
     d.ldgate = _row_stride(gate, "gate")
     return d
+
+
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    """New contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(
+        t.shape, dtype=t.dtype, device=t.device)
 
 
 def _memory(t: torch.Tensor, ld: int):
@@ -1428,45 +1436,46 @@ def residual_norm(y: torch.Tensor, x: Optional[torch.Tensor] = None, *, norm: st
     want_stats: also return the float32 [4, rows] statistics residual_norm_bwd needs.
     out = (h, z): where to write; h may be x and z may be y, in place.  Rows may be strided."""
     d = _block_norm_desc(y, x, gate, gate_act, norm, post, pre, eps)
-    C, rows, dev = d.C, d.rows, y.device
+    C, index = d.C, y.get_device()
     gp = bp = gq = bq = None
     if post is not None:
-        gp = _channel_vector(post[0], C, dev, "post gamma")
-        bp = _channel_vector(post[1], C, dev, "post beta")
+        gp = _channel_vector(post[0], C, index, "post gamma")
+        bp = _channel_vector(post[1], C, index, "post beta")
     if pre is not None:
-        gq = _channel_vector(pre[0], C, dev, "pre gamma")
-        bq = _channel_vector(pre[1], C, dev, "pre beta")
-    xt = y.dtype if x is None else x.dtype
-    h, z = (None, None) if out is None else out
-    if h is None:
-        h = torch.empty(y.shape, dtype=xt, device=dev)
-        d.ldh = C
+        gq = _channel_vector(pre[0], C, index, "pre gamma")
+        bq = _channel_vector(pre[1], C, index, "pre beta")
+    s = _channel_vector(scale, C, index, "scale")
+    like_h = y if x is None else x
+    if out is None:
+        h, z = _dense_like(like_h), None if pre is None else _dense_like(y)
+        d.ldh = d.ldz = C
     else:
-        if h.shape != y.shape or h.dtype != xt or h.device != dev:
-            raise ValueError(f"h must be {xt} {tuple(y.shape)} on {dev}")
-        d.ldh = _row_stride(h, "h")
-    if pre is None:
-        if z is not None:
-            raise ValueError("an output for z without the norm before the next block")
-    elif z is None:
-        z = torch.empty(y.shape, dtype=y.dtype, device=dev)
-        d.ldz = C
-    else:
-        if z.shape != y.shape or z.dtype != y.dtype or z.device != dev:
-            raise ValueError(f"z must be {y.dtype} {tuple(y.shape)} on {dev}")
-        d.ldz = _row_stride(z, "z")
-    if out is not None:
-        for o, ld, own in ((h, d.ldh, x), (z, d.ldz, y)):
-            if o is not None:
-                for t, ldt in ((y, d.ldy), (x, d.ldx), (gate, d.ldgate)):
-                    _refuse_overlap(o, ld, t, ldt, "an output and an input", t is own)
-        _refuse_overlap(h, d.ldh, z, d.ldz, "h and z", False)
-    stats = torch.empty((4, rows), dtype=torch.float32, device=dev) if want_stats else None
+        h, z = _given_outputs(d, out, y, x, gate, like_h, pre is not None)
+    stats = y.new_empty((4, d.rows), dtype=torch.float32) if want_stats else None
     with on_device(y):
-        check(lib().pe_rnorm_fwd(ctypes.addressof(d), y.data_ptr(), _ptr(x), gp, bp,
-                                 _channel_vector(scale, C, dev, "scale"), _ptr(gate), gq, bq,
-                                 h.data_ptr(), _ptr(z), _ptr(stats), _stream(y)))
+        check(lib().pe_rnorm_fwd(ctypes.addressof(d), y.data_ptr(), _ptr(x), gp, bp, s, _ptr(gate),
+                                 gq, bq, h.data_ptr(), _ptr(z), _ptr(stats), _stream(y)))
     return h, z, stats
+
+
+def _given_outputs(d: RnormDesc, out, y, x, gate, like_h, pre: bool):
+    """Checks residual_norm's out = (h, z), makes the one that is None."""
+    h, z = out
+    if z is not None and not pre:
+        raise ValueError("an output for z without the norm before the next block")
+    h = _dense_like(like_h) if h is None else h
+    z = _dense_like(y) if z is None and pre else z
+    for o, like, name in ((h, like_h, "h"), (z, y, "z")):
+        if o is not None:
+            if o.shape != y.shape or o.dtype != like.dtype or o.device != y.device:
+                raise ValueError(f"{name} must be {like.dtype} {tuple(y.shape)} on {y.device}")
+            setattr(d, "ld" + name, _row_stride(o, name))
+    for o, ld, own in ((h, d.ldh, x), (z, d.ldz, y)):
+        if o is not None:
+            for t, ldt in ((y, d.ldy), (x, d.ldx), (gate, d.ldgate)):
+                _refuse_overlap(o, ld, t, ldt, "an output and an input", t is own)
+    _refuse_overlap(h, d.ldh, z, d.ldz, "h and z", False)
+    return h, z
 
 
 def residual_norm_bwd(dh: Optional[torch.Tensor], dz: Optional[torch.Tensor], y: torch.Tensor,
@@ -1484,61 +1493,57 @@ def residual_norm_bwd(dh: Optional[torch.Tensor], dz: Optional[torch.Tensor], y:
     into: tensors of the float32 [C] gradients by name (views of a gradient arena, say), which
     are overwritten.  x and y must hold what forward read: not after h = x or z = y in place."""
     d = _block_norm_desc(y, x, gate, gate_act, norm, post, pre, 1.0)
-    C, rows, dev = d.C, d.rows, y.device
-    xt = y.dtype if x is None else x.dtype
-    _need_gpu(dh, dz, stats)
+    C, rows, index = d.C, d.rows, y.get_device()
     if dh is None and dz is None:
         raise ValueError("neither dh nor dz")
     if (dz is None) != (pre is None):
         raise ValueError("dz is given exactly when there is a norm before the next block")
-    for t, dt, name in ((dh, xt, "dh"), (dz, y.dtype, "dz")):
-        if t is not None:
-            if t.shape != y.shape or t.dtype != dt or t.device != dev:
-                raise ValueError(f"{name} must be {dt} {tuple(y.shape)} on {dev}")
-            setattr(d, "ld" + name, _row_stride(t, name))
+    like_h = y if x is None else x
+    if dh is not None:
+        d.lddh = _incoming(dh, like_h, y, "dh")
+    if dz is not None:
+        d.lddz = _incoming(dz, y, y, "dz")
     if (post is not None or pre is not None) and (
-            stats is None or stats.dtype != torch.float32 or tuple(stats.shape) != (4, rows)
-            or not stats.is_contiguous() or stats.device != dev):
-        raise ValueError(f"stats must be forward's: contiguous float32 [4, {rows}] on {dev}")
-    given = {"dscale": scale, "dpost_gamma": None, "dpost_beta": None, "dpre_gamma": None,
-             "dpre_beta": None}
-    if post is not None:
-        given["dpost_gamma"], given["dpost_beta"] = post
-    if pre is not None:
-        given["dpre_gamma"], given["dpre_beta"] = pre
-    vec = {k: _channel_vector(t, C, dev, k[1:]) for k, t in given.items()}
-    res = {"dy": torch.empty(y.shape, dtype=y.dtype, device=dev),
-           "dx": None if x is None else torch.empty(y.shape, dtype=xt, device=dev),
-           "dgate": None if gate is None else torch.empty(gate.shape, dtype=y.dtype, device=dev)}
+            stats is None or stats.dtype is not torch.float32 or stats.shape != (4, rows)
+            or not stats.is_contiguous() or stats.device != y.device):
+        raise ValueError(f"stats must be forward's: contiguous float32 [4, {rows}] on {y.device}")
+    gp, bp = (None, None) if post is None else post
+    gq, bq = (None, None) if pre is None else pre
+    dy, dx = _dense_like(y), None if x is None else _dense_like(x)
+    dgate = None if gate is None else _dense_like(gate)
     d.lddy = d.lddx = d.lddgate = C
-    into = {} if into is None else into
-    unknown = [k for k in into if given.get(k) is None]
-    if unknown:
-        raise ValueError(f"no such parameter gradients: {unknown}")
-    seen = set()
-    for k, t in given.items():
-        o = into.get(k)
-        if o is None:
-            o = None if t is None else torch.empty(C, dtype=torch.float32, device=dev)
-        else:
-            p = _channel_vector(o, C, dev, k)
-            if p in seen:
-                raise ValueError("two parameter gradients share memory")
-            seen.add(p)
-        res[k] = o
-    need = lib().pe_rnorm_bwd_workspace_bytes(ctypes.addressof(d))
+    grads = {"dscale": scale, "dpost_gamma": gp, "dpost_beta": bp, "dpre_gamma": gq,
+             "dpre_beta": bq}
+    scale, gp, bp, gq, _ = [_channel_vector(t, C, index, k[1:]) for k, t in grads.items()]
+    want = [k for k, t in grads.items() if t is not None]
+    if into:
+        into = {k: o for k, o in into.items() if o is not None}
+        if not into.keys() <= set(want):
+            raise ValueError(f"no such parameter gradients: {sorted(into.keys() - set(want))}")
+        if len({_channel_vector(o, C, index, k) for k, o in into.items()}) < len(into):
+            raise ValueError("two parameter gradients share memory")
+        grads.update(into)
+        want = [k for k in want if k not in into]
+    if want:
+        grads.update(zip(want, y.new_empty((len(want), C), dtype=torch.float32).unbind(0)))
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be contiguous on {dev}")
-    if gate is not None and rows == 0:
-        res["dgate"].zero_()
+        workspace = y.new_empty(lib().pe_rnorm_bwd_workspace_bytes(ctypes.addressof(d)),
+                                dtype=torch.uint8)
+    elif workspace.device != y.device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {y.device}")
+    if dgate is not None and rows == 0:
+        dgate.zero_()
     with on_device(y):
         check(lib().pe_rnorm_bwd(
-            ctypes.addressof(d), _ptr(dh), _ptr(dz), y.data_ptr(), _ptr(x), _ptr(stats),
-            vec["dpost_gamma"], vec["dpost_beta"], vec["dscale"], _ptr(gate), vec["dpre_gamma"],
-            res["dy"].data_ptr(), _ptr(res["dx"]), _ptr(res["dgate"]), _ptr(res["dpost_gamma"]),
-            _ptr(res["dpost_beta"]), _ptr(res["dscale"]), _ptr(res["dpre_gamma"]),
-            _ptr(res["dpre_beta"]), workspace.data_ptr(),
+            ctypes.addressof(d), _ptr(dh), _ptr(dz), y.data_ptr(), _ptr(x), _ptr(stats), gp, bp,
+            scale, _ptr(gate), gq, dy.data_ptr(), _ptr(dx), _ptr(dgate),
+            _ptr(grads["dpost_gamma"]), _ptr(grads["dpost_beta"]), _ptr(grads["dscale"]),
+            _ptr(grads["dpre_gamma"]), _ptr(grads["dpre_beta"]), workspace.data_ptr(),
             workspace.numel() * workspace.element_size(), _stream(y)))
-    return res
+    return {"dy": dy, "dx": dx, "dgate": dgate, **grads}
+
+
+def _incoming(t: torch.Tensor, like: torch.Tensor, y: torch.Tensor, name: str) -> int:
+    if t.shape != y.shape or t.dtype != like.dtype or t.device != y.device:
+        raise ValueError(f"{name} must be {like.dtype} {tuple(y.shape)} on {y.device}")
+    return t.shape[-1] if t.is_contiguous() else _row_stride(t, name)

@@ -11,8 +11,8 @@ import numpy as np
 import torch
 
 from . import _ffi
-from ._ffi import (PE_DTYPE_BF16, PE_DTYPE_F32, PE_NORM_INF, PE_NORM_L2, PE_NORM_MAX_SHARES,
-                   ClipDesc, check, lib)
+from ._ffi import (PE_DTYPE_BF16, PE_DTYPE_F32, PE_NORM_INF, PE_NORM_L2, PE_NORM_FEW_ELEMENTS,
+                   PE_NORM_FEW_SHARES, PE_NORM_MAX_SHARES, ClipDesc, check, lib)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -362,12 +362,12 @@ def adam_step(p: torch.Tensor, m: torch.Tensor, v: torch.Tensor, grad: torch.Ten
     s, a = adam_scalars(lr, beta1, beta2, step, tf1)
     if max_norm is not None:
         d = _clip_desc(max_norm, norm_type, grad_scale, skip_nonfinite, norm_over, p)
-        norm, workspace = _norm_buffers(p.device, None, workspace)
+        norm, workspace, ws = _norm_buffers(p.device, None, workspace, norm_over is None and
+                                            p.numel() <= PE_NORM_FEW_ELEMENTS)
         with on_device(p):
             check(lib().pe_adam_clip_step(p.data_ptr(), m.data_ptr(), v.data_ptr(),
                                           grad.data_ptr(), _ptr(p_bf16), p.numel(), beta1, beta2,
-                                          eps, s, a, ctypes.addressof(d), norm.data_ptr(),
-                                          workspace.data_ptr(), _stream(p)))
+                                          eps, s, a, ctypes.addressof(d), norm.data_ptr(), ws, _stream(p)))
         return norm
     _no_clip(skip_nonfinite, norm_over)
     with on_device(p):
@@ -397,12 +397,12 @@ def sgd_step(p: torch.Tensor, mom: torch.Tensor, grad: torch.Tensor, lr: float,
                                    or p_bf16.numel() != p.numel()):
             raise ValueError("p_bf16 must be contiguous bfloat16 of the same length")
         d = _clip_desc(max_norm, norm_type, grad_scale, skip_nonfinite, norm_over, p)
-        norm, workspace = _norm_buffers(p.device, None, workspace)
+        norm, workspace, ws = _norm_buffers(p.device, None, workspace, norm_over is None and
+                                            p.numel() <= PE_NORM_FEW_ELEMENTS)
         with on_device(p):
             check(lib().pe_sgd_clip_step(p.data_ptr(), mom.data_ptr(), grad.data_ptr(),
                                          _ptr(p_bf16), p.numel(), lr, momentum,
-                                         ctypes.addressof(d), norm.data_ptr(),
-                                         workspace.data_ptr(), _stream(p)))
+                                         ctypes.addressof(d), norm.data_ptr(), ws, _stream(p)))
         return norm
     _no_clip(skip_nonfinite, norm_over)
     with on_device(p):
@@ -422,17 +422,21 @@ def _norm_kind(norm_type: float) -> int:
     raise ValueError(f"norm_type must be 2 or inf, got {norm_type!r}")
 
 
-def _norm_buffers(device, out: Optional[torch.Tensor], workspace: Optional[torch.Tensor]):
+def _norm_buffers(device, out: Optional[torch.Tensor], workspace: Optional[torch.Tensor],
+                  few: bool):
+    """(norm, workspace, workspace's address); a call over few elements needs no workspace."""
     if out is None:
         out = torch.empty(1, dtype=torch.float32, device=device)
     elif out.device != device or out.dtype != torch.float32 or out.numel() != 1:
         raise ValueError(f"the norm goes to one float32 element on {device}")
     if workspace is None:
+        if few:
+            return out, None, None
         workspace = torch.empty(_NORM_WS, dtype=torch.uint8, device=device)
     elif workspace.device != device or not workspace.is_contiguous() or \
             workspace.numel() * workspace.element_size() < _NORM_WS:
         raise ValueError(f"workspace must be contiguous, {_NORM_WS} bytes on {device}")
-    return out, workspace
+    return out, workspace, workspace.data_ptr()
 
 
 _NORM_WS = 2 * PE_NORM_MAX_SHARES   # a float64 for every four shares
@@ -563,11 +567,11 @@ def grad_norm(grads, norm_type: float = 2.0, grad_scale: float = 1.0,
     carry over to the norm."""
     s = _as_set(grads)
     kind = _norm_kind(norm_type)
-    out, workspace = _norm_buffers(s.device, out, workspace)
+    out, workspace, ws = _norm_buffers(s.device, out, workspace, s.shares <= PE_NORM_FEW_SHARES)
     with on_device(out):
         spans, begin, shares = s._on_stream()
-        check(lib().pe_grad_norm(spans, begin, shares, kind, grad_scale, out.data_ptr(),
-                                 workspace.data_ptr(), _stream(out)))
+        check(lib().pe_grad_norm(spans, begin, shares, kind, grad_scale, out.data_ptr(), ws,
+                                 _stream(out)))
     return out
 
 
@@ -584,9 +588,9 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, grad_scale: float
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
-    out, workspace = _norm_buffers(s.device, out, workspace)
+    out, workspace, ws = _norm_buffers(s.device, out, workspace, s.shares <= PE_NORM_FEW_SHARES)
     with on_device(out):
         spans, begin, shares = s._on_stream()
-        check(lib().pe_grad_clip(spans, begin, shares, kind, grad_scale, max_norm, out.data_ptr(),
-                                 workspace.data_ptr(), _stream(out)))
+        check(lib().pe_grad_clip(spans, begin, shares, kind, grad_scale, max_norm, out.data_ptr(), ws,
+                                 _stream(out)))
     return out

@@ -32,7 +32,7 @@ def test_c_entries_refuse_bad_arguments_on_the_host():
     assert lib.pe_grad_norm(one, one, 1, 7, 1.0, one, one, None) == U
     assert lib.pe_grad_norm(one, one, 1, 0, INF, one, one, None) == E
     assert lib.pe_grad_norm(one, one, 1, 0, 1.0, None, one, None) == E
-    assert lib.pe_grad_norm(one, one, 1, 0, 1.0, one, None, None) == E
+    assert lib.pe_grad_norm(one, one, 17, 0, 1.0, one, None, None) == E
     assert lib.pe_grad_norm(one, one, 1, 0, 1.0, one, 20, None) == E
     assert lib.pe_grad_clip(one, one, 1, 0, 1.0, -1.0, one, one, None) == E
     assert lib.pe_grad_clip(one, one, 1, 0, 1.0, math.nan, one, one, None) == E
@@ -45,7 +45,7 @@ def test_c_entries_refuse_bad_arguments_on_the_host():
                                      None)
 
     assert adam(p=None) == E and adam(grad=8) == E and adam(desc=None) == E and adam(n=-1) == E
-    assert adam(norm=None) == E and adam(ws=None) == E and adam(ws=12) == E
+    assert adam(norm=None) == E and adam(ws=None, n=16385) == E and adam(ws=12) == E
     for field, bad, code in (("kind", 3, U), ("grad_scale", math.nan, E), ("max_norm", -2.0, E),
                              ("max_norm", math.nan, E), ("shares", 1, E), ("shares", 5000, E)):
         b = _ffi.ClipDesc(None, None, 1.0, -1, 0, 1.0, 0)
@@ -120,9 +120,9 @@ def test_entry_points_refuse_bad_options(on_cpu):
     with pytest.raises(ValueError):
         ops.sgd_step(v, v, v, 0.1, max_norm=1.0, p_bf16=v)
     with pytest.raises(ValueError):
-        ops._norm_buffers(v.device, torch.zeros(2), None)
+        ops._norm_buffers(v.device, torch.zeros(2), None, False)
     with pytest.raises(ValueError):
-        ops._norm_buffers(v.device, None, torch.zeros(100, dtype=torch.uint8))
+        ops._norm_buffers(v.device, None, torch.zeros(100, dtype=torch.uint8), True)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         pe.nn._need_gpu(v)
 
