@@ -728,8 +728,7 @@ int32_t pe_bn_bwd_bf16(const void* da, const void* a, int32_t relu, const void* 
  * stats (may be NULL in forward) receives [4][rows] float32: mean, rstd of y, mean, rstd of h;
  * the planes of a norm that is off, and the means of an RMS norm, are left as they were.
  * h may be x and z may be y, in place: the same pointer and stride.  C is at most 8192; ld* are
- * row strides in elements; C % 8 == 0 with every pointer and stride a multiple of 16 bytes is the
- * fast layout, any other works.
+ * row strides in elements; pointers and strides need the alignment of an element only.
  *
  * Backward: from dh (may be NULL: 0) and dz (with pre) to dy, dx (may be NULL), dgate (with a
  * gate) and the parameter gradients asked for (overwritten, not added to).  dx may be dh, dy may

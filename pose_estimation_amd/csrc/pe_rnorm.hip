@@ -7,10 +7,12 @@
 // and writes dy and dx, each once: a row lives in the registers of the team of threads that owns
 // it from its load to its store, so statistics, both norms and the gate cost no further pass.
 // Eight channels a thread (one 16-byte load of bf16): a team is the next power of two of C/8
-// threads inside one wave (8 to 64, several rows a wave side by side), or, past 512 channels, a
+// threads inside one wave (1 to 64, several rows a wave side by side), or, past 512 channels, a
 // workgroup of its own.  Means and variances are taken in two steps from the registers (no
 // difference of large sums), all arithmetic is float32, each output is rounded once.
 #include <math.h>
+
+#include <initializer_list>
 
 #include "pe_common.h"
 
@@ -23,7 +25,10 @@ constexpr int kRnThreads = 256;   // of a workgroup whose rows are shorter than 
 // 256 bf16 the launch takes 141, 129, 133, 145, 138 us with 256, 512, 768, 1024, 2048 of them, at
 // 3456 x 2048 29, 26, 28, 30, 35 us, and the fold behind it grows with their number.
 constexpr int kRnItems = 512;
-enum { kQ1 = 1, kQ0 = 2, kP1 = 4, kP0 = 8 };   // which sums of backward anything needs
+// The sums an item leaves, as bits of what anything needs: of dz*hhat, dz, D*phi*yhat and D*phi,
+// and with a gate shared by several rows also of D*yhat and D.
+enum { kQ1 = 1, kQ0 = 2, kP1 = 4, kP0 = 8, kG1 = 16, kG0 = 32 };
+constexpr int slots_of(long gate_rows) { return gate_rows > 1 ? 6 : 4; }
 
 struct RnFwd {
     const void *y, *x, *gate;
@@ -33,6 +38,7 @@ struct RnFwd {
     long rows, gate_rows;      // rows per gate row; 0 = no gate
     long ldy, ldx, ldg, ldh, ldz;
     long rows_blk;
+    double inv_c64;
     float eps, inv_c;
     int C, post, pre, layer, act;
 };
@@ -41,8 +47,8 @@ struct RnBwd {
     const void *dh, *dz, *y, *x, *gate;
     const float *stats, *gp, *bp, *s, *gq;
     void *dy, *dx, *dgate;
-    float* part;               // [items][4][pitch]: sums of dz*hhat, dz, D*phi*yhat, D*phi
-    int pitch, need;           // which of them are stored
+    float* part;               // [items][slots][pitch]
+    int pitch, need;
     long rows, gate_rows;
     long lddh, lddz, ldy, ldx, ldg, lddy, lddx, lddg;
     long group, nseg, rows_blk;   // rows of a group, items of a group, rows of an item
@@ -53,7 +59,7 @@ struct RnBwd {
 // ---- a thread's eight channels ------------------------------------------------------------
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-// TEAM: the threads of a row inside a wave (8 to 64), or the most that a workgroup working on one
+// TEAM: the threads of a row inside a wave (1 to 64), or the most that a workgroup working on one
 // row has (512, 1024: so many registers a thread can have).
 __host__ __device__ constexpr bool in_wave(int team) { return team <= 64; }
 
@@ -62,12 +68,31 @@ __device__ __forceinline__ int team_size() {
     return in_wave(TEAM) ? TEAM : (int)blockDim.x;
 }
 
-// VEC: channels 8t .. 8t+7 in 16-byte accesses.  Otherwise t, t + T, t + 2T, ...: any C, any
-// alignment, still coalesced.
-template <bool VEC>
-__device__ __forceinline__ int channel(int t, int T, int j) {
-    return VEC ? t * kRnEl + j : t + j * T;
-}
+// How a row's channels lie over its threads.  WHOLE (C a multiple of 8): thread t has channels 8t
+// to 8t+7.  TAIL: the last thread has the row's last eight, which the one before it shares: it
+// computes them all and counts and stores only those from `first` on, so that no load needs a
+// branch of its own (which would make the wave wait for it).  FEW (C < 8): one channel a thread.
+// Rows start at any element: 16-byte accesses need no alignment here.
+enum { WHOLE, TAIL, FEW };
+
+template <int MODE>
+struct Cols {
+    int c, first;
+    bool on;
+    __device__ __forceinline__ Cols(int t, int C) {
+        on = t * (MODE == FEW ? 1 : kRnEl) < C;
+        c = MODE == FEW ? t : t * kRnEl;
+        first = 0;
+        if (MODE == TAIL && c > C - kRnEl) {
+            first = c - (C - kRnEl);
+            c = C - kRnEl;
+        }
+    }
+    // Whether the thread's j-th value is a channel of its own.
+    __device__ __forceinline__ bool mine(int j) const {
+        return on && (MODE == WHOLE || (MODE == TAIL && j >= first) || (MODE == FEW && j == 0));
+    }
+};
 
 __device__ __forceinline__ f32x8 splat(float v) { return f32x8{v, v, v, v, v, v, v, v}; }
 
@@ -75,34 +100,26 @@ __device__ __forceinline__ f32x8 fma8(f32x8 a, f32x8 b, f32x8 c) {
     return __builtin_elementwise_fma(a, b, c);
 }
 
-// A row's channels as they come from memory, so that the next row can be on its way in few
-// registers while this one is worked on.  Channels past C read as 0.
-template <typename T, bool VEC>
-struct Raw {
-    f32x8 f;
-    __device__ __forceinline__ void load(const T* p, int t, int team, int C) {
-        f = splat(0.0f);
-#pragma unroll
-        for (int j = 0; j < kRnEl; ++j)
-            if (t + j * team < C) {
-                if (sizeof(T) == 4) {
-                    f[j] = p[t + j * team];
-                } else {
-                    f[j] = bf16_bits_to_float(p[t + j * team]);
-                }
-            }
-    }
-    __device__ __forceinline__ f32x8 value() const { return f; }
-};
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
-template <>
-struct Raw<float, true> {
+// A row's channels as they come from memory, so that the next row can be on its way in few
+// registers while this one is worked on.  Threads without channels read as 0.
+template <typename T, int MODE>
+struct Raw;
+
+template <int MODE>
+struct Raw<float, MODE> {
     f32x4 a, b;
-    __device__ __forceinline__ void load(const float* p, int t, int, int C) {
+    __device__ __forceinline__ void load(const float* p, const Cols<MODE>& k, bool use = true) {
         a = b = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (t * kRnEl < C) {
-            a = *reinterpret_cast<const f32x4*>(p + t * kRnEl);
-            b = *reinterpret_cast<const f32x4*>(p + t * kRnEl + 4);
+        if (use && k.on) {
+            if (MODE == FEW) {
+                a.x = p[k.c];
+            } else {
+                a = *reinterpret_cast<const f32x4_any*>(p + k.c);
+                b = *reinterpret_cast<const f32x4_any*>(p + k.c + 4);
+            }
         }
     }
     __device__ __forceinline__ f32x8 value() const {
@@ -110,12 +127,18 @@ struct Raw<float, true> {
     }
 };
 
-template <>
-struct Raw<uint16_t, true> {
+template <int MODE>
+struct Raw<uint16_t, MODE> {
     u32x4 v;
-    __device__ __forceinline__ void load(const uint16_t* p, int t, int, int C) {
+    __device__ __forceinline__ void load(const uint16_t* p, const Cols<MODE>& k, bool use = true) {
         v = u32x4{0, 0, 0, 0};
-        if (t * kRnEl < C) v = *reinterpret_cast<const u32x4*>(p + t * kRnEl);
+        if (use && k.on) {
+            if (MODE == FEW) {
+                v.x = p[k.c];
+            } else {
+                v = *reinterpret_cast<const u32x4_any*>(p + k.c);
+            }
+        }
     }
     __device__ __forceinline__ f32x8 value() const {
         f32x8 f;
@@ -128,62 +151,53 @@ struct Raw<uint16_t, true> {
     }
 };
 
-template <bool VEC, typename T>
-__device__ __forceinline__ f32x8 load8(const T* p, int t, int team, int C) {
-    Raw<T, VEC> r;
-    r.load(p, t, team, C);
+template <int MODE, typename T>
+__device__ __forceinline__ f32x8 load8(const T* p, const Cols<MODE>& k) {
+    Raw<T, MODE> r;
+    r.load(p, k);
     return r.value();
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store8(float* p, int t, int T, int C, f32x8 f) {
-    if (VEC) {
-        if (t * kRnEl < C) {
-            *reinterpret_cast<f32x4*>(p + t * kRnEl) = f32x4{f[0], f[1], f[2], f[3]};
-            *reinterpret_cast<f32x4*>(p + t * kRnEl + 4) = f32x4{f[4], f[5], f[6], f[7]};
-        }
-    } else {
+template <int MODE>
+__device__ __forceinline__ void store8(float* p, const Cols<MODE>& k, f32x8 f) {
+    if (MODE != FEW && k.on && k.first == 0) {
+        *reinterpret_cast<f32x4_any*>(p + k.c) = f32x4{f[0], f[1], f[2], f[3]};
+        *reinterpret_cast<f32x4_any*>(p + k.c + 4) = f32x4{f[4], f[5], f[6], f[7]};
+    } else if (MODE != WHOLE) {
 #pragma unroll
         for (int j = 0; j < kRnEl; ++j)
-            if (t + j * T < C) p[t + j * T] = f[j];
+            if (k.mine(j)) p[k.c + j] = f[j];
     }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store8(uint16_t* p, int t, int T, int C, f32x8 f) {
-    if (VEC) {
-        if (t * kRnEl < C) {
-            u32x4 v;
+template <int MODE>
+__device__ __forceinline__ void store8(uint16_t* p, const Cols<MODE>& k, f32x8 f) {
+    u32x4 v;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = pack_bf16x2_bits(f[2 * j], f[2 * j + 1]);
-            *reinterpret_cast<u32x4*>(p + t * kRnEl) = v;
-        }
-    } else {
+    for (int j = 0; j < 4; ++j) v[j] = pack_bf16x2_bits(f[2 * j], f[2 * j + 1]);
+    if (MODE != FEW && k.on && k.first == 0) {
+        *reinterpret_cast<u32x4_any*>(p + k.c) = v;
+    } else if (MODE != WHOLE) {
 #pragma unroll
         for (int j = 0; j < kRnEl; ++j)
-            if (t + j * T < C) p[t + j * T] = (uint16_t)float_to_bf16_bits(f[j]);
+            if (k.mine(j)) p[k.c + j] = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
     }
 }
 
-template <bool VEC>
-__device__ __forceinline__ f32x8 load_param(const float* p, float absent, int t, int T, int C) {
-    return p ? load8<VEC>(p, t, T, C) : splat(absent);
+template <int MODE>
+__device__ __forceinline__ f32x8 load_param(const float* p, float absent, const Cols<MODE>& k) {
+    return p ? load8<MODE>(p, k) : splat(absent);
 }
 
 __device__ __forceinline__ float sum8(f32x8 v) {
     return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
 }
 
-// 0 in the place of channels past C.
-template <bool VEC>
-__device__ __forceinline__ f32x8 inside(f32x8 v, int t, int T, int C) {
-    if (VEC) {
-        if (t * kRnEl >= C) v = splat(0.0f);
-    } else {
+// 0 in the place of channels that are not the thread's own.
+template <int MODE>
+__device__ __forceinline__ f32x8 inside(f32x8 v, const Cols<MODE>& k) {
 #pragma unroll
-        for (int j = 0; j < kRnEl; ++j)
-            if (t + j * T >= C) v[j] = 0.0f;
-    }
+    for (int j = 0; j < kRnEl; ++j) v[j] = k.mine(j) ? v[j] : 0.0f;
     return v;
 }
 
@@ -199,9 +213,9 @@ __device__ __forceinline__ float dpp_add(float v) {
 
 template <int W>
 __device__ __forceinline__ float lanes_sum(float v) {
-    v = dpp_add<0xB1>(v);    // quad_perm 1 0 3 2
-    v = dpp_add<0x4E>(v);    // quad_perm 2 3 0 1
-    v = dpp_add<0x141>(v);   // row_half_mirror
+    if (W >= 2) v = dpp_add<0xB1>(v);     // quad_perm 1 0 3 2
+    if (W >= 4) v = dpp_add<0x4E>(v);     // quad_perm 2 3 0 1
+    if (W >= 8) v = dpp_add<0x141>(v);    // row_half_mirror
     if (W >= 16) v = dpp_add<0x140>(v);   // row_mirror
     if (W >= 32) {
         const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -214,54 +228,125 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
+__device__ __forceinline__ double join64(unsigned lo, unsigned hi) {
+    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
+}
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+    const unsigned long long x = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)x, CTRL, 0xf, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(x >> 32), CTRL, 0xf, 0xf, true);
+    return v + join64((unsigned)lo, (unsigned)hi);
+}
+
+// a summed over the wave's halves in its lower half, b in its upper one.
+__device__ __forceinline__ double add_halves(double a, double b) {
+    const unsigned long long x = __double_as_longlong(a), y = __double_as_longlong(b);
+    const auto lo = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)y, false, false);
+    const auto hi = __builtin_amdgcn_permlane32_swap((unsigned)(x >> 32), (unsigned)(y >> 32), false, false);
+    return join64(lo[0], hi[0]) + join64(lo[1], hi[1]);
+}
+
+// a summed over pairs of rows of 16 lanes in the even rows, b in the odd ones.
+__device__ __forceinline__ double add_rows(double a, double b) {
+    const unsigned long long x = __double_as_longlong(a), y = __double_as_longlong(b);
+    const auto lo = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)y, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap((unsigned)(x >> 32), (unsigned)(y >> 32), false, false);
+    return join64(lo[0], hi[0]) + join64(lo[1], hi[1]);
+}
+
+// Of the whole wave.
+__device__ __forceinline__ double lanes_sum64(double v) {
+    v = dpp_add<0x140>(dpp_add<0x141>(dpp_add<0x4E>(dpp_add<0xB1>(v))));
+    v = add_rows(v, v);
+    return add_halves(v, v);
+}
+
 // A workgroup as a team: the waves' sums through LDS in order; two buffers in turn, so one
 // barrier a sum is enough.
 struct TeamSums {
-    float2* buf;   // LDS [2][16], workgroup teams only
+    double2* buf;   // LDS [2][16], workgroup teams only
     int turn;
+    double inv_c;   // 1 / C, forward only
 };
+
+template <typename T2, typename T>
+__device__ __forceinline__ void waves_sum2(T& a, T& b, TeamSums& ts) {
+    T2* buf = reinterpret_cast<T2*>(ts.buf + 16 * ts.turn);
+    ts.turn ^= 1;
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = T2{a, b};
+    __syncthreads();
+    const int waves = (int)blockDim.x >> 6;
+    T2 v = buf[0];
+    for (int i = 1; i < waves; ++i) {
+        v.x += buf[i].x;
+        v.y += buf[i].y;
+    }
+    a = v.x;
+    b = v.y;
+}
 
 template <int TEAM>
 __device__ __forceinline__ void team_sum2(float& a, float& b, TeamSums& ts) {
     constexpr int W = in_wave(TEAM) ? TEAM : 64;
     a = lanes_sum<W>(a);
     b = lanes_sum<W>(b);
-    if (!in_wave(TEAM)) {
-        float2* buf = ts.buf + 16 * ts.turn;
-        ts.turn ^= 1;
-        if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = make_float2(a, b);
-        __syncthreads();
-        const int waves = (int)blockDim.x >> 6;
-        float2 v = buf[0];
-        for (int i = 1; i < waves; ++i) {
-            v.x += buf[i].x;
-            v.y += buf[i].y;
-        }
-        a = v.x;
-        b = v.y;
-    }
+    if (!in_wave(TEAM)) waves_sum2<float2>(a, b, ts);
 }
 
-// mean and rstd of the row, v replaced by the normalised row (anything past C).
-template <int TEAM, bool VEC>
-__device__ __forceinline__ void normalise(f32x8& v, int t, int T, int C, float inv_c, float eps,
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float a, TeamSums& ts) {
+    a = lanes_sum<in_wave(TEAM) ? TEAM : 64>(a);
+    float unused = 0.0f;
+    if (!in_wave(TEAM)) waves_sum2<float2>(a, unused, ts);
+    return a;
+}
+
+// mean and rstd of the row, v replaced by the normalised row.  Inside a wave mean and variance
+// are taken one after the other.  A workgroup would pay a barrier for each: it sums values and
+// squares together in float64, where the squares of float32 are exact and their difference
+// from the mean's square is good to 2^-53 of the larger.
+template <int TEAM, int MODE>
+__device__ __forceinline__ void normalise(f32x8& v, const Cols<MODE>& k, float inv_c, float eps,
                                           bool layer, float& mean, float& rstd, TeamSums& ts) {
     mean = 0.0f;
-    float unused = 0.0f;
-    if (layer) {
-        float sum = sum8(v);   // channels past C hold 0
-        team_sum2<TEAM>(sum, unused, ts);
-        mean = sum * inv_c;
+    float var;
+    if (layer && !in_wave(TEAM)) {
+        const f32x8 in = inside<MODE>(v, k);
+        double s1 = 0.0, s2 = 0.0;
+#pragma unroll
+        for (int j = 0; j < kRnEl; ++j) {
+            const double x = (double)in[j];
+            s1 += x;
+            s2 = __builtin_fma(x, x, s2);
+        }
+        s1 = lanes_sum64(s1);
+        s2 = lanes_sum64(s2);
+        waves_sum2<double2>(s1, s2, ts);
+        const double m = s1 * ts.inv_c;
+        mean = (float)m;
+        var = (float)__builtin_fma(-m, m, s2 * ts.inv_c);
+        if (var < 0.0f) var = 0.0f;   // NaN stays
         v -= mean;
+    } else {
+        if (layer) {
+            mean = team_sum<TEAM>(sum8(inside<MODE>(v, k)), ts) * inv_c;
+            v -= mean;
+        }
+        const f32x8 in = inside<MODE>(v, k);
+        var = team_sum<TEAM>(sum8(in * in), ts) * inv_c;
     }
-    const f32x8 in = inside<VEC>(v, t, T, C);
-    float sq = sum8(in * in);
-    team_sum2<TEAM>(sq, unused, ts);
-    rstd = 1.0f / sqrtf(sq * inv_c + eps);
+    rstd = 1.0f / sqrtf(var + eps);
     v *= rstd;
 }
 
 // ---- gate ---------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float as_float(T v) {
+    return sizeof(T) == 4 ? (float)v : bf16_bits_to_float((uint32_t)v);
+}
+
 __device__ __forceinline__ float sigmoid(float g) {
     return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
 }
@@ -291,60 +376,74 @@ __device__ __forceinline__ void gate8(f32x8 g, int act, f32x8& phi, f32x8& slope
 }
 
 __device__ __forceinline__ long gate_row(long row, long per) {
-    if (per == 1) return row;
     if (row <= 0x7fffffffl && per <= 0x7fffffffl) return (long)((unsigned)row / (unsigned)per);
     return row / per;
 }
 
 // ---- forward ------------------------------------------------------------------------------
-template <typename YT, typename XT, int TEAM, bool VEC>
+// OWN: a gate row for each row.  The next row is loaded while this one is worked on.
+template <typename YT, typename XT, bool OWN, int MODE>
+struct FwdRow {
+    Raw<YT, MODE> y, gate;
+    Raw<XT, MODE> x;
+    __device__ __forceinline__ void load(const RnFwd& a, long row, const Cols<MODE>& k) {
+        y.load(static_cast<const YT*>(a.y) + row * a.ldy, k);
+        x.load(static_cast<const XT*>(a.x) + row * a.ldx, k, a.x);
+        if (OWN) gate.load(static_cast<const YT*>(a.gate) + row * a.ldg, k);
+    }
+};
+
+template <typename YT, typename XT, bool OWN, int TEAM, int MODE>
 __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_kernel(RnFwd a) {
-    __shared__ float2 lds[in_wave(TEAM) ? 1 : 32];
-    TeamSums ts{lds, 0};
+    __shared__ double2 lds[in_wave(TEAM) ? 1 : 32];
+    TeamSums ts{lds, 0, a.inv_c64};
     const int T = team_size<TEAM>();
     const int t = in_wave(TEAM) ? (int)threadIdx.x % T : (int)threadIdx.x;
     const int teams = in_wave(TEAM) ? kRnThreads / T : 1;
-    const int C = a.C;
-    const f32x8 s = load_param<VEC>(a.s, 1.0f, t, T, C);
-    const f32x8 A = load_param<VEC>(a.gp, 1.0f, t, T, C) * s;
-    const f32x8 B = load_param<VEC>(a.bp, 0.0f, t, T, C) * s;
-    const f32x8 gq = load_param<VEC>(a.gq, 1.0f, t, T, C);
-    const f32x8 bq = load_param<VEC>(a.bq, 0.0f, t, T, C);
-    f32x8 phi = splat(1.0f), slope;
+    const Cols<MODE> k(t, a.C);
     const long lo = (long)blockIdx.x * a.rows_blk;
     const long hi = lo + a.rows_blk < a.rows ? lo + a.rows_blk : a.rows;
+    long row = lo + (in_wave(TEAM) ? (int)threadIdx.x / T : 0);
+    FwdRow<YT, XT, OWN, MODE> now, next;
+    if (row < hi) now.load(a, row, k);
+    const f32x8 s = load_param<MODE>(a.s, 1.0f, k);
+    const f32x8 A = load_param<MODE>(a.gp, 1.0f, k) * s;
+    const f32x8 B = load_param<MODE>(a.bp, 0.0f, k) * s;
+    const f32x8 gq = load_param<MODE>(a.gq, 1.0f, k);
+    const f32x8 bq = load_param<MODE>(a.bq, 0.0f, k);
+    f32x8 phi = splat(1.0f), slope;
     long have = -1;   // the gate row phi holds
-    for (long row = lo + (in_wave(TEAM) ? (int)threadIdx.x / T : 0); row < hi; row += teams) {
-        f32x8 y = load8<VEC>(static_cast<const YT*>(a.y) + row * a.ldy, t, T, C);
-        f32x8 h = splat(0.0f);
-        if (a.x) h = load8<VEC>(static_cast<const XT*>(a.x) + row * a.ldx, t, T, C);
-        if (a.gate_rows) {
+    for (; row < hi; row += teams) {
+        if (row + teams < hi) next.load(a, row + teams, k);
+        f32x8 y = now.y.value(), h = now.x.value();
+        if (OWN) {
+            gate8(now.gate.value(), a.act, phi, slope);
+        } else if (a.gate_rows) {
             const long g = gate_row(row, a.gate_rows);
             if (g != have) {
-                gate8(load8<VEC>(static_cast<const YT*>(a.gate) + g * a.ldg, t, T, C), a.act, phi,
-                      slope);
+                gate8(load8<MODE>(static_cast<const YT*>(a.gate) + g * a.ldg, k), a.act, phi, slope);
                 have = g;
             }
         }
         float mean, rstd;
         if (a.post) {
-            normalise<TEAM, VEC>(y, t, T, C, a.inv_c, a.eps, a.layer, mean, rstd, ts);
+            normalise<TEAM, MODE>(y, k, a.inv_c, a.eps, a.layer, mean, rstd, ts);
             if (a.stats && t == 0) {
                 if (a.layer) a.stats[row] = mean;
                 a.stats[a.rows + row] = rstd;
             }
         }
         h = fma8(fma8(y, A, B), phi, h);
-        store8<VEC>(static_cast<XT*>(a.h) + row * a.ldh, t, T, C, h);
+        store8<MODE>(static_cast<XT*>(a.h) + row * a.ldh, k, h);
         if (a.pre) {
-            h = inside<VEC>(h, t, T, C);
-            normalise<TEAM, VEC>(h, t, T, C, a.inv_c, a.eps, a.layer, mean, rstd, ts);
+            normalise<TEAM, MODE>(h, k, a.inv_c, a.eps, a.layer, mean, rstd, ts);
             if (a.stats && t == 0) {
                 if (a.layer) a.stats[2 * a.rows + row] = mean;
                 a.stats[3 * a.rows + row] = rstd;
             }
-            store8<VEC>(static_cast<YT*>(a.z) + row * a.ldz, t, T, C, fma8(h, gq, bq));
+            store8<MODE>(static_cast<YT*>(a.z) + row * a.ldz, k, fma8(h, gq, bq));
         }
+        now = next;
     }
 }
 
@@ -359,21 +458,20 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_k
 // items in order in float64, so the results have the same bits on every call.  An item never
 // crosses a gate row: phi is a constant of the item and is left out of its sums (the fold knows
 // the item's gate), unless the gate has a row for each row, whose gradient needs no sum.
-template <typename YT, typename XT, bool OWN, bool VEC>
+template <typename YT, typename XT, bool OWN, int MODE>
 struct RnRow {
-    Raw<YT, VEC> y, dz, gate;
-    Raw<XT, VEC> x, dh;
+    Raw<YT, MODE> y, dz, gate;
+    Raw<XT, MODE> x, dh;
     float py, ry, ph, rh;   // mean and rstd of y and of h
     // What is absent reads as 0 (x, dh) or is not looked at (the rest).
-    __device__ __forceinline__ void load(const RnBwd& a, long row, int t, int T) {
-        const int C = a.C;
-        y.load(static_cast<const YT*>(a.y) + row * a.ldy, t, T, C);
-        x.load(static_cast<const XT*>(a.x) + row * a.ldx, t, T, a.x && a.pre ? C : 0);
-        dh.load(static_cast<const XT*>(a.dh) + row * a.lddh, t, T, a.dh ? C : 0);
+    __device__ __forceinline__ void load(const RnBwd& a, long row, const Cols<MODE>& k) {
+        y.load(static_cast<const YT*>(a.y) + row * a.ldy, k);
+        x.load(static_cast<const XT*>(a.x) + row * a.ldx, k, a.x && a.pre);
+        dh.load(static_cast<const XT*>(a.dh) + row * a.lddh, k, a.dh);
         py = ph = 0.0f;
         ry = rh = 1.0f;
         if (a.pre) {
-            dz.load(static_cast<const YT*>(a.dz) + row * a.lddz, t, T, C);
+            dz.load(static_cast<const YT*>(a.dz) + row * a.lddz, k);
             rh = a.stats[3 * a.rows + row];
             if (a.layer) ph = a.stats[2 * a.rows + row];
         }
@@ -381,59 +479,85 @@ struct RnRow {
             ry = a.stats[a.rows + row];
             if (a.layer) py = a.stats[row];
         }
-        if (OWN) gate.load(static_cast<const YT*>(a.gate) + row * a.ldg, t, T, C);
+        if (OWN) gate.load(static_cast<const YT*>(a.gate) + row * a.ldg, k);
     }
 };
 
-// OWN: a gate row for each row.  The next row is loaded while this one is worked on, except by
-// workgroups of more than 512 threads, which have no registers for it.
-template <typename YT, typename XT, bool OWN, int TEAM, bool VEC>
+// OWN: a gate row for each row.  The next row is loaded while this one is worked on.  Workgroups
+// of more than 512 threads, which have 128 registers a thread, keep the parameters in LDS.
+template <typename YT, typename XT, bool OWN, int TEAM, int MODE>
 __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_kernel(RnBwd a) {
-    __shared__ float2 lds[in_wave(TEAM) ? 1 : 32];
+    __shared__ double2 lds[in_wave(TEAM) ? 1 : 32];
     __shared__ float fold[in_wave(TEAM) ? kRnThreads / 64 : 1][4][in_wave(TEAM) ? TEAM * kRnEl : 1];
-    TeamSums ts{lds, 0};
+    TeamSums ts{lds, 0, 0.0};
     const int T = team_size<TEAM>();
     const int t = in_wave(TEAM) ? (int)threadIdx.x % T : (int)threadIdx.x;
     const int teams = in_wave(TEAM) ? kRnThreads / T : 1;
-    const int C = a.C;
-    const f32x8 s = load_param<VEC>(a.s, 1.0f, t, T, C);
-    const f32x8 A = load_param<VEC>(a.gp, 1.0f, t, T, C) * s;
-    const f32x8 B = load_param<VEC>(a.bp, 0.0f, t, T, C) * s;
-    const f32x8 gq = load_param<VEC>(a.gq, 1.0f, t, T, C);
+    const Cols<MODE> k(t, a.C);
+    constexpr bool WIDE = TEAM == 1024;
+    __shared__ f32x4 held[WIDE ? 6 : 1][WIDE ? 1024 : 1];   // each thread's own, no barrier
+    const f32x8 s = load_param<MODE>(a.s, 1.0f, k);
+    f32x8 A = load_param<MODE>(a.gp, 1.0f, k) * s;
+    f32x8 B = load_param<MODE>(a.bp, 0.0f, k) * s;
+    f32x8 gq = load_param<MODE>(a.gq, 1.0f, k);
+    auto hold = [&](int i, f32x8 v) {
+        held[2 * i][threadIdx.x] = v.lo;
+        held[2 * i + 1][threadIdx.x] = v.hi;
+    };
+    auto held8 = [&](int i) {
+        f32x8 v;
+        v.lo = held[2 * i][threadIdx.x];
+        v.hi = held[2 * i + 1][threadIdx.x];
+        return v;
+    };
+    if (WIDE) {
+        hold(0, A);
+        hold(1, B);
+        hold(2, gq);
+    }
     f32x8 phi = splat(1.0f), slope = splat(1.0f);
     const long g = (long)blockIdx.x / a.nseg;
     const long lo = g * a.group + ((long)blockIdx.x - g * a.nseg) * a.rows_blk;
     const long end = (g + 1) * a.group;
     const long hi = lo + a.rows_blk < end ? lo + a.rows_blk : end;
     if (!OWN && a.gate_rows)
-        gate8(load8<VEC>(static_cast<const YT*>(a.gate) + g * a.ldg, t, T, C), a.act, phi, slope);
+        gate8(load8<MODE>(static_cast<const YT*>(a.gate) + g * a.ldg, k), a.act, phi, slope);
     f32x8 q1 = splat(0.0f), q0 = q1, p1 = q1, p0 = q1;
     long row = lo + (in_wave(TEAM) ? (int)threadIdx.x / T : 0);
-    RnRow<YT, XT, OWN, VEC> now, next;
-    constexpr bool AHEAD = TEAM != 1024;
-    if (AHEAD && row < hi) now.load(a, row, t, T);
+    RnRow<YT, XT, OWN, MODE> now, next;
+    if (row < hi) now.load(a, row, k);
     for (; row < hi; row += teams) {
-        if (!AHEAD) now.load(a, row, t, T);
-        if (AHEAD && row + teams < hi) next.load(a, row + teams, t, T);
+        if (row + teams < hi) next.load(a, row + teams, k);
         f32x8 y = now.y.value(), d = now.dh.value();
         if (OWN) gate8(now.gate.value(), a.act, phi, slope);
         if (a.post) y = (y - now.py) * now.ry;
         if (a.pre) {
+            if (WIDE) {
+                A = held8(0);
+                B = held8(1);
+                gq = held8(2);
+            }
             f32x8 w = now.dz.value();
             const f32x8 hhat = (fma8(fma8(y, A, B), phi, now.x.value()) - now.ph) * now.rh;
             q0 += w;
             q1 = fma8(w, hhat, q1);
-            w *= gq;
+            w = inside<MODE>(w * gq, k);
             float m1 = sum8(w), m2 = sum8(w * hhat);
             team_sum2<TEAM>(m1, m2, ts);
             m1 = a.layer ? m1 * a.inv_c : 0.0f;
             m2 *= a.inv_c;
             d = fma8(fma8(hhat, splat(-m2), w - m1), splat(now.rh), d);
         }
-        if (a.dx) store8<VEC>(static_cast<XT*>(a.dx) + row * a.lddx, t, T, C, d);
-        if (OWN)
-            store8<VEC>(static_cast<YT*>(a.dgate) + row * a.lddg, t, T, C, d * fma8(y, A, B) * slope);
-        d = inside<VEC>(d, t, T, C);
+        if (a.dx) store8<MODE>(static_cast<XT*>(a.dx) + row * a.lddx, k, d);
+        if (WIDE) A = held8(0);
+        if (OWN) {
+            if (WIDE) {   // again, rather than kept over the sum
+                B = held8(1);
+                gate8(now.gate.value(), a.act, phi, slope);
+            }
+            store8<MODE>(static_cast<YT*>(a.dgate) + row * a.lddg, k, d * fma8(y, A, B) * slope);
+        }
+        d = inside<MODE>(d, k);
         const f32x8 u = d * phi;
         const f32x8 keep = OWN ? u : d;
         p0 += keep;
@@ -446,106 +570,93 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
             n2 *= a.inv_c;
             w = fma8(y, splat(-n2), w - n1) * now.ry;
         }
-        store8<VEC>(static_cast<YT*>(a.dy) + row * a.lddy, t, T, C, w);
-        if (AHEAD) now = next;
+        store8<MODE>(static_cast<YT*>(a.dy) + row * a.lddy, k, w);
+        now = next;
     }
     if (!a.need) return;
-    float* out = a.part + (long)blockIdx.x * 4 * a.pitch;
+    const bool shared = !OWN && a.gate_rows;
+    float* out = a.part + (long)blockIdx.x * slots_of(a.gate_rows) * a.pitch;
     if (in_wave(TEAM)) {
         // rows side by side in the wave, then the waves in order
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const f32x8 sums = k == 0 ? q1 : k == 1 ? q0 : k == 2 ? p1 : p0;
-            if (a.need & (1 << k)) {
+        for (int i = 0; i < 4; ++i) {
+            const f32x8 sums = i == 0 ? q1 : i == 1 ? q0 : i == 2 ? p1 : p0;
+            if (a.need & ((1 << i) | (i >= 2 ? 4 << i : 0))) {
 #pragma unroll
                 for (int j = 0; j < kRnEl; ++j) {
                     float v = sums[j];
 #pragma unroll
                     for (int off = 32; off >= (in_wave(TEAM) ? TEAM : 64); off >>= 1)
                         v += __shfl_xor(v, off, 64);
-                    if ((int)(threadIdx.x & 63) < T)
-                        fold[threadIdx.x >> 6][k][channel<VEC>(t, T, j)] = v;
+                    if ((int)(threadIdx.x & 63) < T && k.mine(j)) fold[threadIdx.x >> 6][i][k.c + j] = v;
                 }
             }
         }
         __syncthreads();
+        for (int c = threadIdx.x; c < a.C; c += kRnThreads) {
+            float f = 1.0f, unused;
+            if (shared) f = gate_value(as_float(static_cast<const YT*>(a.gate)[g * a.ldg + c]), a.act, unused);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (a.need & (1 << k)) {
-                for (int c = threadIdx.x; c < C; c += kRnThreads) {
-                    float v = fold[0][k][c];
+            for (int i = 0; i < 4; ++i) {
+                const bool weighted = a.need & (1 << i), plain = i >= 2 && (a.need & (4 << i));
+                if (weighted || plain) {
+                    float v = fold[0][i][c];
 #pragma unroll
-                    for (int wv = 1; wv < kRnThreads / 64; ++wv) v += fold[wv][k][c];
-                    out[(long)k * a.pitch + c] = v;
+                    for (int wv = 1; wv < kRnThreads / 64; ++wv) v += fold[wv][i][c];
+                    if (weighted) out[(long)i * a.pitch + c] = i >= 2 ? v * f : v;
+                    if (plain) out[(long)(i + 2) * a.pitch + c] = v;
                 }
             }
         }
     } else {
-        if (a.need & kQ1) store8<VEC>(out, t, T, C, q1);
-        if (a.need & kQ0) store8<VEC>(out + a.pitch, t, T, C, q0);
-        if (a.need & kP1) store8<VEC>(out + 2l * a.pitch, t, T, C, p1);
-        if (a.need & kP0) store8<VEC>(out + 3l * a.pitch, t, T, C, p0);
+        const f32x8 f = shared ? phi : splat(1.0f);
+        if (a.need & kQ1) store8<MODE>(out, k, q1);
+        if (a.need & kQ0) store8<MODE>(out + a.pitch, k, q0);
+        if (a.need & kP1) store8<MODE>(out + 2l * a.pitch, k, p1 * f);
+        if (a.need & kP0) store8<MODE>(out + 3l * a.pitch, k, p0 * f);
+        if (a.need & kG1) store8<MODE>(out + 4l * a.pitch, k, p1);
+        if (a.need & kG0) store8<MODE>(out + 5l * a.pitch, k, p0);
     }
 }
 
 // ---- fold of the items --------------------------------------------------------------------
 // Latency is all there is to it: a few MB that were just written.  A workgroup takes 32 channels
-// (a 128-byte line of every row of sums), a thread four of them of every LANES-th item, with the
+// (a 128-byte line of every row of sums), a thread four of them of every 32nd item, with the
 // loads of several items under way at a time; float64 sums in an order fixed by the sizes.
+// Workgroups of one launch have one of two tasks: a gate row's gradient from its own items, or
+// the parameters' from all of them (whose sums phi weights already).
 constexpr int kFoldCols = 32;
-constexpr int kFoldMany = 32;    // items side by side
-constexpr int kFoldFew = 8;      // the same where a gate row has few
+constexpr int kFoldLanes = 32;                        // items side by side
+constexpr int kFoldThreads = kFoldLanes * kFoldCols / 4;
+// Items that one workgroup of the parameters folds.  Past it (a gate row for every few rows of a
+// long tensor) kFoldSlices of them leave their sums behind the items for a second launch.
+constexpr long kFoldItems = 4096;
+constexpr int kFoldSlices = 64;
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 struct RnFold {
     float* part;
-    long items, step;          // this fold's items: 0, step, 2*step, ...
+    long items, nseg;                // items in all and of a gate row
+    long first;                      // gate row of the grid's first
+    int gates, slices;               // tasks of the grid: gate rows, then slices of the parameters
     const float *gp, *bp, *s, *any;
     const void* gate;
     void* dgate;
     float *dgp, *dbp, *ds, *dgq, *dbq;
-    long nseg, ldg, lddg;
-    int C, act, pitch, need;
+    long ldg, lddg;
+    int C, act, pitch, need, slots;
 };
 
-__device__ __forceinline__ double join64(unsigned lo, unsigned hi) {
-    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
-}
-
-// a summed over the wave's halves in its lower half, b in its upper one.
-__device__ __forceinline__ double add_halves(double a, double b) {
-    const unsigned long long x = __double_as_longlong(a), y = __double_as_longlong(b);
-    const auto lo = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)y, false, false);
-    const auto hi = __builtin_amdgcn_permlane32_swap((unsigned)(x >> 32), (unsigned)(y >> 32), false, false);
-    return join64(lo[0], hi[0]) + join64(lo[1], hi[1]);
-}
-
-// a summed over pairs of rows of 16 lanes in the even rows, b in the odd ones.
-__device__ __forceinline__ double add_rows(double a, double b) {
-    const unsigned long long x = __double_as_longlong(a), y = __double_as_longlong(b);
-    const auto lo = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)y, false, false);
-    const auto hi = __builtin_amdgcn_permlane16_swap((unsigned)(x >> 32), (unsigned)(y >> 32), false, false);
-    return join64(lo[0], hi[0]) + join64(lo[1], hi[1]);
-}
-
-// v + v of the lane eight further in its row of 16.
-__device__ __forceinline__ double add_eight(double v) {
-    const unsigned long long x = __double_as_longlong(v);
-    const int lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)x, 0x128, 0xf, 0xf, true);
-    const int hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(x >> 32), 0x128, 0xf, 0xf, true);
-    return v + join64((unsigned)lo, (unsigned)hi);
-}
-
-// sum[k] of channel c = sum over i < n of part[(first + i*step)][k][c], in the first kFoldCols
-// threads, whose channel is the block's first plus their index.
-template <int LANES>
-__device__ __forceinline__ void fold_items(const RnFold& a, long first, long n, long step,
-                                           double (&sum)[4]) {
+// sum[k] of channel c = sum over lo <= i < hi of part[i][slot + k][c], k < K, in the first
+// kFoldCols threads, whose channel is the block's first plus their index.
+template <int K>
+__device__ __forceinline__ void fold_items(const RnFold& a, long lo, long hi, int slot, double (&sum)[4]) {
     constexpr int QUADS = kFoldCols / 4;
-    constexpr int WAVES = LANES * QUADS / 64;
+    constexpr int WAVES = kFoldThreads / 64;
     constexpr int AT_ONCE = 4;
     static_assert(QUADS == 8, "the sums over a wave's lanes");
     __shared__ double lds[WAVES][4][kFoldCols];
+    const int need = a.need >> slot;
     const int quad = (int)threadIdx.x % QUADS, lane = (int)threadIdx.x / QUADS;
     const int c = (int)blockIdx.x * kFoldCols + quad * 4;
     f64x4 v[4];
@@ -554,36 +665,36 @@ __device__ __forceinline__ void fold_items(const RnFold& a, long first, long n, 
     if (c < a.pitch) {
         // A branch around a load would make the thread wait for each in turn: items past the end
         // read the last one again and count as 0, sums that nothing needs read one that is.
-        const float* p = a.part + first * 4 * a.pitch + c;
-        const long jump = step * 4 * a.pitch;
-        const int any = __builtin_ctz(a.need);
-        long at[4];
+        const long jump = (long)a.slots * a.pitch;
+        const int any = __builtin_ctz(need);
+        long at[K];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) at[k] = (long)((a.need & (1 << k)) ? k : any) * a.pitch;
-        for (long i = lane; i < n; i += AT_ONCE * LANES) {
-            f32x4 r[AT_ONCE][4];
+        for (int k = 0; k < K; ++k) at[k] = (long)(slot + ((need & (1 << k)) ? k : any)) * a.pitch + c;
+        for (long i = lo + lane; i < hi; i += AT_ONCE * kFoldLanes) {
+            f32x4 r[AT_ONCE][K];
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u) {
-                const float* q = p + (i + u * LANES < n ? i + u * LANES : n - 1) * jump;
+                const float* q = a.part + (i + u * kFoldLanes < hi ? i + u * kFoldLanes : hi - 1) * jump;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) r[u][k] = *reinterpret_cast<const f32x4*>(q + at[k]);
+                for (int k = 0; k < K; ++k) r[u][k] = *reinterpret_cast<const f32x4*>(q + at[k]);
             }
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u) {
-                const bool in = i + u * LANES < n;
+                const bool in = i + u * kFoldLanes < hi;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                for (int k = 0; k < K; ++k) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[k][j] += (double)(in ? r[u][k][j] : 0.0f);
                 }
             }
         }
     }
-    // a wave's eight items into one: each step leaves half of the sums to half of the lanes
+    // a wave's eight items into one: each step leaves half of the sums to half of the lanes; the
+    // last adds the lane eight further in its row of 16
     const int l = (int)threadIdx.x & 63, k = 2 * ((l >> 4) & 1) + (l >> 5);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const double u = add_eight(add_rows(add_halves(v[0][j], v[1][j]), add_halves(v[2][j], v[3][j])));
+        const double u = dpp_add<0x128>(add_rows(add_halves(v[0][j], v[1][j]), add_halves(v[2][j], v[3][j])));
         if ((l & 15) < QUADS) lds[threadIdx.x >> 6][k][quad * 4 + j] = u;
     }
     __syncthreads();
@@ -593,74 +704,64 @@ __device__ __forceinline__ void fold_items(const RnFold& a, long first, long n, 
             sum[k] = lds[0][k][threadIdx.x];
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) sum[k] += lds[w][k][threadIdx.x];
+            if (!(need & (1 << k))) sum[k] = 0.0;
         }
     }
 }
 
-// A channel's parameters, asked for before the sums; again no branch around a load, an absent one
-// reads a.any.
-struct FoldParam {
-    float gp, bp, s;
-    __device__ __forceinline__ FoldParam(const RnFold& a, int c)
-        : gp(*(a.gp ? a.gp + c : a.any)), bp(*(a.bp ? a.bp + c : a.any)), s(*(a.s ? a.s + c : a.any)) {}
-    __device__ __forceinline__ void settle(const RnFold& a) {
+template <typename YT, bool GROUPED>
+__global__ __launch_bounds__(kFoldThreads) void rnorm_fold_kernel(RnFold a) {
+    const int c = (int)blockIdx.x * kFoldCols + (int)threadIdx.x;
+    const bool mine = threadIdx.x < kFoldCols && c < a.C;
+    const int at = mine ? c : 0;
+    // the channel's parameters, asked for before the sums; an absent one reads a.any
+    float gp = *(a.gp ? a.gp + at : a.any), bp = *(a.bp ? a.bp + at : a.any);
+    float s = *(a.s ? a.s + at : a.any);
+    double v[4];
+    if (GROUPED && (int)blockIdx.y < a.gates) {
+        const long g = a.first + blockIdx.y;
+        const YT raw = static_cast<const YT*>(a.gate)[g * a.ldg + at];
+        fold_items<2>(a, g * a.nseg, (g + 1) * a.nseg, 4, v);
+        if (!mine) return;
         if (!a.gp) gp = 1.0f;
         if (!a.bp) bp = 0.0f;
         if (!a.s) s = 1.0f;
-    }
-};
-
-// One gate row: its gradient, and its sums with phi in place of its first item's.
-template <typename YT, int LANES>
-__global__ __launch_bounds__(LANES * kFoldCols / 4) void rnorm_fold_gate_kernel(RnFold a) {
-    const long g = blockIdx.y;
-    const int c = (int)blockIdx.x * kFoldCols + (int)threadIdx.x;
-    const bool mine = threadIdx.x < kFoldCols && c < a.C;
-    FoldParam par(a, mine ? c : 0);
-    const YT raw = static_cast<const YT*>(a.gate)[g * a.ldg + (mine ? c : 0)];
-    double v[4];
-    fold_items<LANES>(a, g * a.nseg, a.nseg, 1, v);
-    if (mine) {
-        par.settle(a);
-        const float gv = sizeof(YT) == 4 ? (float)raw : bf16_bits_to_float((uint32_t)raw);
         float slope;
-        const float phi = gate_value(gv, a.act, slope);
-        const double gp = par.gp, bp = par.bp, s = par.s;
-        const float dg = (float)((double)slope * s * (gp * v[2] + bp * v[3]));
+        gate_value(as_float(raw), a.act, slope);
+        const float dg = (float)((double)slope * s * ((double)gp * v[0] + (double)bp * v[1]));
         if (sizeof(YT) == 4) {
             static_cast<float*>(a.dgate)[g * a.lddg + c] = dg;
         } else {
             static_cast<uint16_t*>(a.dgate)[g * a.lddg + c] = (uint16_t)float_to_bf16_bits(dg);
         }
-        float* p = a.part + g * a.nseg * 4 * a.pitch + c;
-        p[0] = (float)v[0];
-        p[a.pitch] = (float)v[1];
-        p[2l * a.pitch] = (float)(v[2] * phi);
-        p[3l * a.pitch] = (float)(v[3] * phi);
+        return;
     }
-}
-
-__global__ __launch_bounds__(kFoldMany * kFoldCols / 4) void rnorm_fold_kernel(RnFold a) {
-    const int c = (int)blockIdx.x * kFoldCols + (int)threadIdx.x;
-    const bool mine = threadIdx.x < kFoldCols && c < a.C;
-    FoldParam par(a, mine ? c : 0);
-    double v[4];
-    fold_items<kFoldMany>(a, 0, a.items, a.step, v);
-    if (mine) {
-        par.settle(a);
-        const double gp = par.gp, bp = par.bp, s = par.s;
-        if (a.dgq) a.dgq[c] = (float)v[0];
-        if (a.dbq) a.dbq[c] = (float)v[1];
-        if (a.dgp) a.dgp[c] = (float)(s * v[2]);
-        if (a.dbp) a.dbp[c] = (float)(s * v[3]);
-        if (a.ds) a.ds[c] = (float)(gp * v[2] + bp * v[3]);
+    const int slice = (int)blockIdx.y - a.gates;
+    const long per = (a.items + a.slices - 1) / a.slices;
+    const long lo = slice * per, hi = lo + per < a.items ? lo + per : a.items;
+    fold_items<4>(a, lo, hi, 0, v);
+    if (!mine) return;
+    if (a.slices > 1) {
+        float* p = a.part + a.items * a.slots * a.pitch + slice * 4l * a.pitch + c;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[(long)k * a.pitch] = (float)v[k];
+        return;
     }
+    if (!a.gp) gp = 1.0f;
+    if (!a.bp) bp = 0.0f;
+    if (!a.s) s = 1.0f;
+    if (a.dgq) a.dgq[c] = (float)v[0];
+    if (a.dbq) a.dbq[c] = (float)v[1];
+    if (a.dgp) a.dgp[c] = (float)((double)s * v[2]);
+    if (a.dbp) a.dbp[c] = (float)((double)s * v[3]);
+    if (a.ds) a.ds[c] = (float)((double)gp * v[2] + (double)bp * v[3]);
 }
 
 // ---- host ---------------------------------------------------------------------------------
 static int team_of(int C) {
     const int need = (C + kRnEl - 1) / kRnEl;
-    for (int t = 8; t <= 64; t *= 2)
+    if (C < kRnEl) return 8;   // a channel a thread
+    for (int t = 1; t <= 64; t *= 2)
         if (need <= t) return t;
     return need <= 512 ? 512 : 1024;
 }
@@ -694,8 +795,10 @@ static BwdGeom bwd_geom(const pe_rnorm_desc& d) {
     return g;
 }
 
-static bool vec_ok(const void* p, long ld, int dtype) {
-    return aligned(p, 16) && (ld * (dtype == PE_DTYPE_F32 ? 4 : 2)) % 16 == 0;
+static bool element_aligned(int dtype, std::initializer_list<const void*> ptrs) {
+    for (const void* p : ptrs)
+        if (!aligned(p, dtype == PE_DTYPE_F32 ? 4 : 2)) return false;
+    return true;
 }
 
 static int32_t check_desc(const char* what, const pe_rnorm_desc* d) {
@@ -721,59 +824,85 @@ static int32_t check_desc(const char* what, const pe_rnorm_desc* d) {
     return PE_OK;
 }
 
-// Calls F<TEAM, VEC>::go(args) for the team and layout at hand.
-template <template <int, bool> class F, class... A>
-static void with_team(int team, bool vec, A&&... a) {
-    switch (team) {
-        case 8: vec ? F<8, true>::go(a...) : F<8, false>::go(a...); break;
-        case 16: vec ? F<16, true>::go(a...) : F<16, false>::go(a...); break;
-        case 32: vec ? F<32, true>::go(a...) : F<32, false>::go(a...); break;
-        case 64: vec ? F<64, true>::go(a...) : F<64, false>::go(a...); break;
-        case 512: vec ? F<512, true>::go(a...) : F<512, false>::go(a...); break;
-        default: vec ? F<1024, true>::go(a...) : F<1024, false>::go(a...);
+// Calls F<TEAM, MODE>::go(args) for C channels.
+template <template <int, int> class F, class... A>
+static void with_team(int C, A&&... a) {
+    if (C < kRnEl) return F<8, FEW>::go(a...);
+    const bool whole = C % kRnEl == 0;
+    switch (team_of(C)) {
+        case 1: return F<1, WHOLE>::go(a...);   // eight channels
+        case 2: return whole ? F<2, WHOLE>::go(a...) : F<2, TAIL>::go(a...);
+        case 4: return whole ? F<4, WHOLE>::go(a...) : F<4, TAIL>::go(a...);
+        case 8: return whole ? F<8, WHOLE>::go(a...) : F<8, TAIL>::go(a...);
+        case 16: return whole ? F<16, WHOLE>::go(a...) : F<16, TAIL>::go(a...);
+        case 32: return whole ? F<32, WHOLE>::go(a...) : F<32, TAIL>::go(a...);
+        case 64: return whole ? F<64, WHOLE>::go(a...) : F<64, TAIL>::go(a...);
+        case 512: return whole ? F<512, WHOLE>::go(a...) : F<512, TAIL>::go(a...);
+        default: return whole ? F<1024, WHOLE>::go(a...) : F<1024, TAIL>::go(a...);
     }
 }
 
-template <typename YT, typename XT>
+template <typename YT, typename XT, bool OWN>
 struct FwdOf {
-    template <int TEAM, bool VEC>
+    template <int TEAM, int MODE>
     struct F {
-        static void go(const RnFwd& a, unsigned blocks, unsigned threads, hipStream_t st) {
-            launch(rnorm_fwd_kernel<YT, XT, TEAM, VEC>, blocks, threads, 0, st, a);
+        static void go(const RnFwd& a, unsigned blocks, hipStream_t st) {
+            launch(rnorm_fwd_kernel<YT, XT, OWN, TEAM, MODE>, blocks, block_of(a.C), 0, st, a);
         }
     };
 };
 
 template <typename YT, typename XT, bool OWN>
 struct BwdOf {
-    template <int TEAM, bool VEC>
+    template <int TEAM, int MODE>
     struct F {
-        static void go(const RnBwd& a, unsigned blocks, unsigned threads, hipStream_t st) {
-            launch(rnorm_bwd_kernel<YT, XT, OWN, TEAM, VEC>, blocks, threads, 0, st, a);
+        static void go(const RnBwd& a, unsigned blocks, hipStream_t st) {
+            launch(rnorm_bwd_kernel<YT, XT, OWN, TEAM, MODE>, blocks, block_of(a.C), 0, st, a);
         }
     };
 };
 
 template <typename YT, typename XT>
-static void launch_bwd(const RnBwd& a, bool vec, unsigned blocks, hipStream_t st) {
+static void launch_bwd(const RnBwd& a, unsigned blocks, hipStream_t st) {
     if (a.gate_rows == 1) {
-        with_team<BwdOf<YT, XT, true>::template F>(team_of(a.C), vec, a, blocks, block_of(a.C), st);
+        with_team<BwdOf<YT, XT, true>::template F>(a.C, a, blocks, st);
     } else {
-        with_team<BwdOf<YT, XT, false>::template F>(team_of(a.C), vec, a, blocks, block_of(a.C), st);
+        with_team<BwdOf<YT, XT, false>::template F>(a.C, a, blocks, st);
     }
 }
 
 template <typename YT, typename XT>
-static void launch_fwd(const RnFwd& a, bool vec, unsigned blocks, hipStream_t st) {
-    with_team<FwdOf<YT, XT>::template F>(team_of(a.C), vec, a, blocks, block_of(a.C), st);
+static void launch_fwd(const RnFwd& a, unsigned blocks, hipStream_t st) {
+    if (a.gate_rows == 1) {
+        with_team<FwdOf<YT, XT, true>::template F>(a.C, a, blocks, st);
+    } else {
+        with_team<FwdOf<YT, XT, false>::template F>(a.C, a, blocks, st);
+    }
 }
 
+// Gate rows (65535 tasks a grid at most) and the parameters in one launch where their items allow.
 template <typename YT>
-static void launch_fold_gate(const RnFold& a, bool few, dim3 grid, hipStream_t st) {
-    if (few) {
-        launch(rnorm_fold_gate_kernel<YT, kFoldFew>, grid, kFoldFew * kFoldCols / 4, 0, st, a);
-    } else {
-        launch(rnorm_fold_gate_kernel<YT, kFoldMany>, grid, kFoldMany * kFoldCols / 4, 0, st, a);
+static void launch_fold(RnFold f, bool grouped, long groups, bool params, hipStream_t st) {
+    const unsigned tiles = (unsigned)((f.C + kFoldCols - 1) / kFoldCols);
+    const int slices = !params ? 0 : f.items > kFoldItems ? kFoldSlices : 1;
+    f.slices = slices > 1 ? slices : 1;
+    if (!grouped) {
+        f.gates = 0;
+        launch(rnorm_fold_kernel<YT, false>, tiles, kFoldThreads, 0, st, f);
+        return;
+    }
+    for (f.first = 0; f.first < groups; f.first += f.gates) {
+        f.gates = (int)(groups - f.first < 60000 ? groups - f.first : 60000);
+        const unsigned more = f.first == 0 ? (unsigned)slices : 0;
+        launch(rnorm_fold_kernel<YT, true>, dim3(tiles, (unsigned)f.gates + more), kFoldThreads, 0, st, f);
+    }
+    if (slices > 1) {
+        f.part += f.items * f.slots * f.pitch;
+        f.items = slices;
+        f.slots = 4;
+        f.slices = 1;
+        f.gates = 0;
+        launch(rnorm_fold_kernel<YT, false>, tiles, kFoldThreads, 0, st, f);
     }
 }
 
@@ -795,6 +924,9 @@ extern "C" int32_t pe_rnorm_fwd(const pe_rnorm_desc* d, const void* y, const voi
     PE_REQUIRE(d->gate_rows == 0 || gate, PE_E_INVALID, "pe_rnorm_fwd: NULL gate");
     PE_REQUIRE(d->post || !(post_gamma || post_beta), PE_E_INVALID,
                "pe_rnorm_fwd: parameters of a norm that is off");
+    PE_REQUIRE(element_aligned(d->y_dtype, {y, gate, z}) && element_aligned(d->x_dtype, {x, h}) &&
+                   element_aligned(PE_DTYPE_F32, {post_gamma, post_beta, scale, pre_gamma, pre_beta, stats}),
+               PE_E_INVALID, "pe_rnorm_fwd: a pointer between two elements");
     RnFwd a;
     a.y = y;
     a.x = x;
@@ -816,34 +948,51 @@ extern "C" int32_t pe_rnorm_fwd(const pe_rnorm_desc* d, const void* y, const voi
     a.ldz = d->ldz;
     a.eps = d->eps;
     a.inv_c = 1.0f / (float)d->C;
+    a.inv_c64 = 1.0 / (double)d->C;
     a.C = d->C;
     a.post = d->post;
     a.pre = d->pre;
     a.layer = d->norm == PE_RNORM_LAYER;
     a.act = d->gate_act;
-    const bool vec = d->C % kRnEl == 0 && vec_ok(y, d->ldy, d->y_dtype) && vec_ok(x, d->ldx, d->x_dtype) &&
-                     vec_ok(gate, gate ? d->ldgate : 0, d->y_dtype) && vec_ok(h, d->ldh, d->x_dtype) &&
-                     (!d->pre || vec_ok(z, d->ldz, d->y_dtype)) && aligned(post_gamma, 16) &&
-                     aligned(post_beta, 16) && aligned(scale, 16) && aligned(pre_gamma, 16) &&
-                     aligned(pre_beta, 16);
+    // Workgroups of equal shares, each of which loads the parameters once.  Rows inside a wave:
+    // 4096 of them (60000 x 333 bf16: 47 us, with 8192 51, with 2048 46; 196608 x 256 with a gate
+    // 83, 83, 83).  A row to a workgroup: whole rounds of what the chip holds at once, four (8192 x
+    // 4096 with a float32 residual, rms: 90 us, with two 94), or two or one where the parameters
+    // would be over half of the bytes (8000 x 4000 bf16, layer: two 62 us, four 66).
     const long at_once = rows_at_once(d->C);
-    long rows = (d->rows + 2047) / 2048;
+    long rows = (d->rows + 4095) / 4096;
+    if (!in_wave(team_of(d->C))) {
+        const long round = (1l << 18) / block_of(d->C);
+        const long yb = d->y_dtype == PE_DTYPE_F32 ? 4 : 2, xb = d->x_dtype == PE_DTYPE_F32 ? 4 : 2;
+        const long params = 4 * ((post_gamma != nullptr) + (post_beta != nullptr) + (scale != nullptr) +
+                                 (pre_gamma != nullptr) + (pre_beta != nullptr));
+        const long row = yb + xb + (x ? xb : 0) + (d->pre ? yb : 0) + (d->gate_rows == 1 ? yb : 0);
+        long rounds = 4;
+        do {
+            rows = (d->rows + rounds * round - 1) / (rounds * round);
+            rounds /= 2;
+        } while (rounds && rows * row < 2 * params);
+    }
     rows = (rows + at_once - 1) / at_once * at_once;
     a.rows_blk = rows;
     const unsigned blocks = (unsigned)((d->rows + rows - 1) / rows);
     if (d->y_dtype == PE_DTYPE_F32) {
-        launch_fwd<float, float>(a, vec, blocks, as_stream(stream));
+        launch_fwd<float, float>(a, blocks, as_stream(stream));
     } else if (d->x_dtype == PE_DTYPE_F32) {
-        launch_fwd<uint16_t, float>(a, vec, blocks, as_stream(stream));
+        launch_fwd<uint16_t, float>(a, blocks, as_stream(stream));
     } else {
-        launch_fwd<uint16_t, uint16_t>(a, vec, blocks, as_stream(stream));
+        launch_fwd<uint16_t, uint16_t>(a, blocks, as_stream(stream));
     }
     return check_launch("pe_rnorm_fwd");
 }
 
 extern "C" size_t pe_rnorm_bwd_workspace_bytes(const pe_rnorm_desc* d) {
     if (pe::check_desc("pe_rnorm_bwd_workspace_bytes", d) != PE_OK) return 0;
-    return sizeof(float) * 4 * (size_t)pe::pitch_of(d->C) * (size_t)(d->rows ? pe::bwd_geom(*d).items() : 0);
+    if (d->rows == 0) return 0;
+    const long items = pe::bwd_geom(*d).items();
+    const long slices = items > pe::kFoldItems ? pe::kFoldSlices : 0;
+    return sizeof(float) * (size_t)pe::pitch_of(d->C) *
+           (size_t)(items * pe::slots_of(d->gate_rows) + 4 * slices);
 }
 
 extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const void* dz,
@@ -863,12 +1012,16 @@ extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const vo
                "pe_rnorm_bwd: gradients of a norm that is off");
     PE_REQUIRE(d->pre || !(dpre_gamma || dpre_beta || dz), PE_E_INVALID,
                "pe_rnorm_bwd: gradients of a norm that is off");
+    PE_REQUIRE(element_aligned(d->y_dtype, {dz, y, gate, dy, dgate}) &&
+                   element_aligned(d->x_dtype, {dh, x, dx}) &&
+                   element_aligned(PE_DTYPE_F32, {stats, post_gamma, post_beta, scale, pre_gamma, dpost_gamma,
+                                                  dpost_beta, dscale, dpre_gamma, dpre_beta}),
+               PE_E_INVALID, "pe_rnorm_bwd: a pointer between two elements");
     const bool grouped = d->gate_rows > 1;
     const bool sums = dpost_gamma || dpost_beta || dscale || dpre_gamma || dpre_beta;
-    const bool needs_p1 = dpost_gamma || dscale || grouped;
-    const bool needs_p0 = dpost_beta || ((dscale || grouped) && post_beta);
-    const int need = (dpre_gamma ? kQ1 : 0) | (dpre_beta ? kQ0 : 0) | (needs_p1 ? kP1 : 0) |
-                     (needs_p0 ? kP0 : 0);
+    const int need = (dpre_gamma ? kQ1 : 0) | (dpre_beta ? kQ0 : 0) | (dpost_gamma || dscale ? kP1 : 0) |
+                     (dpost_beta || (dscale && post_beta) ? kP0 : 0) | (grouped ? kG1 : 0) |
+                     (grouped && post_beta ? kG0 : 0);
     BwdGeom g{0, 0, 0, 0};
     if (d->rows) {
         PE_REQUIRE(y && dy, PE_E_INVALID, "pe_rnorm_bwd: NULL y or dy");
@@ -926,19 +1079,13 @@ extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const vo
         a.layer = d->norm == PE_RNORM_LAYER;
         a.act = d->gate_act;
         const int yd = d->y_dtype, xd = d->x_dtype;
-        const bool vec = d->C % kRnEl == 0 && vec_ok(y, d->ldy, yd) && vec_ok(x, x ? d->ldx : 0, xd) &&
-                         vec_ok(dh, dh ? d->lddh : 0, xd) && vec_ok(dz, dz ? d->lddz : 0, yd) &&
-                         vec_ok(gate, gate ? d->ldgate : 0, yd) &&
-                         vec_ok(dgate, dgate ? d->lddgate : 0, yd) && vec_ok(dy, d->lddy, yd) &&
-                         vec_ok(dx, dx ? d->lddx : 0, xd) && aligned(post_gamma, 16) &&
-                         aligned(post_beta, 16) && aligned(scale, 16) && aligned(pre_gamma, 16);
         const unsigned items = (unsigned)g.items();
         if (yd == PE_DTYPE_F32) {
-            launch_bwd<float, float>(a, vec, items, as_stream(stream));
+            launch_bwd<float, float>(a, items, as_stream(stream));
         } else if (xd == PE_DTYPE_F32) {
-            launch_bwd<uint16_t, float>(a, vec, items, as_stream(stream));
+            launch_bwd<uint16_t, float>(a, items, as_stream(stream));
         } else {
-            launch_bwd<uint16_t, uint16_t>(a, vec, items, as_stream(stream));
+            launch_bwd<uint16_t, uint16_t>(a, items, as_stream(stream));
         }
     }
     if (!sums && !(grouped && d->rows)) return check_launch("pe_rnorm_bwd");
@@ -958,35 +1105,19 @@ extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const vo
                            (const float*)dpost_beta, (const float*)dscale, (const float*)dpre_gamma,
                            (const float*)dpre_beta})
         if (!f.any) f.any = q;
+    f.items = g.items();
     f.nseg = g.nseg;
-    f.ldg = d->ldgate;
-    f.lddg = d->lddgate;
     f.C = d->C;
     f.act = d->gate_act;
     f.pitch = pitch_of(d->C);
     f.need = need;
-    f.items = g.items();
-    f.step = 1;
-    const unsigned tiles = (unsigned)((d->C + kFoldCols - 1) / kFoldCols);
-    if (grouped && d->rows) {
-        for (long first = 0; first < g.groups; first += 65535) {   // a grid's y extent
-            RnFold part = f;
-            const long n = g.groups - first < 65535 ? g.groups - first : 65535;
-            part.part += first * g.nseg * 4 * f.pitch;
-            const long e = d->y_dtype == PE_DTYPE_F32 ? 4 : 2;
-            part.gate = static_cast<const char*>(gate) + first * d->ldgate * e;
-            part.dgate = static_cast<char*>(dgate) + first * d->lddgate * e;
-            const dim3 grid(tiles, (unsigned)n);
-            const bool few = g.nseg <= 4 * kFoldFew;   // one round of loads
-            if (d->y_dtype == PE_DTYPE_F32) {
-                launch_fold_gate<float>(part, few, grid, as_stream(stream));
-            } else {
-                launch_fold_gate<uint16_t>(part, few, grid, as_stream(stream));
-            }
-        }
-        f.items = g.groups;
-        f.step = g.nseg;
+    f.slots = slots_of(d->gate_rows);
+    f.ldg = d->ldgate;
+    f.lddg = d->lddgate;
+    if (d->y_dtype == PE_DTYPE_F32) {
+        launch_fold<float>(f, grouped && d->rows, g.groups, sums, as_stream(stream));
+    } else {
+        launch_fold<uint16_t>(f, grouped && d->rows, g.groups, sums, as_stream(stream));
     }
-    if (sums) launch(rnorm_fold_kernel, tiles, kFoldMany * kFoldCols / 4, 0, as_stream(stream), f);
     return check_launch("pe_rnorm_bwd");
 }
