@@ -3,6 +3,7 @@
 #pragma once
 
 #include "pe_common.h"
+#include "pe_lanes.h"
 
 namespace pe {
 
@@ -34,9 +35,7 @@ __device__ __forceinline__ double norm_combine(double a, double b, int kind) {
 
 // The wave's values as one, the same bits in every lane.
 __device__ __forceinline__ double norm_wave(double v, int kind) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v = norm_combine(v, __shfl_xor(v, off, 64), kind);
-    return v;
+    return lanes_all<64>(v, [kind](double a, double b) { return norm_combine(a, b, kind); });
 }
 
 // The workgroup's values as one, the same bits in every thread and on every call: butterfly
@@ -147,8 +146,18 @@ __device__ __forceinline__ void norm_span(const T* __restrict__ at, int n, int l
 // passes and leaves nothing to clear or to count.
 __device__ __forceinline__ double norm_fold(const double* __restrict__ part, int parts,
                                             const ClipRule& r) {
-    double v = 0.0;
-    for (int i = threadIdx.x; i < parts; i += kNormThreads) v = norm_combine(v, part[i], r.kind);
+    constexpr int EACH = kNormMaxParts / kNormThreads;
+    double got[EACH], v = 0.0;
+    if (parts > 0) {
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+            const int i = (int)threadIdx.x + u * kNormThreads;
+            got[u] = part[i < parts ? i : parts - 1];
+        }
+#pragma unroll
+        for (int u = 0; u < EACH; ++u)
+            if ((int)threadIdx.x + u * kNormThreads < parts) v = norm_combine(v, got[u], r.kind);
+    }
     return norm_of(norm_block<kNormThreads>(v, r.kind), r);
 }
 

@@ -15,6 +15,7 @@
 #include <initializer_list>
 
 #include "pe_common.h"
+#include "pe_lanes.h"
 
 namespace pe {
 
@@ -202,67 +203,6 @@ __device__ __forceinline__ f32x8 inside(f32x8 v, const Cols<MODE>& k) {
 }
 
 // ---- sums over a row's team ---------------------------------------------------------------
-// The lanes of a wave by data-parallel moves inside the vector unit, no LDS round trips: lane ^ 1
-// and ^ 2 inside a quad, then mirrors of 8 and of 16 lanes (whose quads agree by then), then
-// swaps of rows of 16 and of halves of the wave.  Every lane of the team ends with the same bits.
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float v) {
-    return v + __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL,
-                                                                     0xf, 0xf, true));
-}
-
-template <int W>
-__device__ __forceinline__ float lanes_sum(float v) {
-    if (W >= 2) v = dpp_add<0xB1>(v);     // quad_perm 1 0 3 2
-    if (W >= 4) v = dpp_add<0x4E>(v);     // quad_perm 2 3 0 1
-    if (W >= 8) v = dpp_add<0x141>(v);    // row_half_mirror
-    if (W >= 16) v = dpp_add<0x140>(v);   // row_mirror
-    if (W >= 32) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-    if (W >= 64) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-    return v;
-}
-
-__device__ __forceinline__ double join64(unsigned lo, unsigned hi) {
-    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
-}
-
-template <int CTRL>
-__device__ __forceinline__ double dpp_add(double v) {
-    const unsigned long long x = __double_as_longlong(v);
-    const int lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)x, CTRL, 0xf, 0xf, true);
-    const int hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(x >> 32), CTRL, 0xf, 0xf, true);
-    return v + join64((unsigned)lo, (unsigned)hi);
-}
-
-// a summed over the wave's halves in its lower half, b in its upper one.
-__device__ __forceinline__ double add_halves(double a, double b) {
-    const unsigned long long x = __double_as_longlong(a), y = __double_as_longlong(b);
-    const auto lo = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)y, false, false);
-    const auto hi = __builtin_amdgcn_permlane32_swap((unsigned)(x >> 32), (unsigned)(y >> 32), false, false);
-    return join64(lo[0], hi[0]) + join64(lo[1], hi[1]);
-}
-
-// a summed over pairs of rows of 16 lanes in the even rows, b in the odd ones.
-__device__ __forceinline__ double add_rows(double a, double b) {
-    const unsigned long long x = __double_as_longlong(a), y = __double_as_longlong(b);
-    const auto lo = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)y, false, false);
-    const auto hi = __builtin_amdgcn_permlane16_swap((unsigned)(x >> 32), (unsigned)(y >> 32), false, false);
-    return join64(lo[0], hi[0]) + join64(lo[1], hi[1]);
-}
-
-// Of the whole wave.
-__device__ __forceinline__ double lanes_sum64(double v) {
-    v = dpp_add<0x140>(dpp_add<0x141>(dpp_add<0x4E>(dpp_add<0xB1>(v))));
-    v = add_rows(v, v);
-    return add_halves(v, v);
-}
-
 // A workgroup as a team: the waves' sums through LDS in order; two buffers in turn, so one
 // barrier a sum is enough.
 struct TeamSums {
@@ -321,8 +261,8 @@ __device__ __forceinline__ void normalise(f32x8& v, const Cols<MODE>& k, float i
             s1 += x;
             s2 = __builtin_fma(x, x, s2);
         }
-        s1 = lanes_sum64(s1);
-        s2 = lanes_sum64(s2);
+        s1 = lanes_sum<64>(s1);
+        s2 = lanes_sum<64>(s2);
         waves_sum2<double2>(s1, s2, ts);
         const double m = s1 * ts.inv_c;
         mean = (float)m;
@@ -694,7 +634,14 @@ __device__ __forceinline__ void fold_items(const RnFold& a, long lo, long hi, in
     const int l = (int)threadIdx.x & 63, k = 2 * ((l >> 4) & 1) + (l >> 5);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const double u = dpp_add<0x128>(add_rows(add_halves(v[0][j], v[1][j]), add_halves(v[2][j], v[3][j])));
+        double x = v[0][j], x2 = v[1][j], y = v[2][j], y2 = v[3][j];
+        swap_halves(x, x2);
+        swap_halves(y, y2);
+        x += x2;
+        y += y2;
+        swap_rows(x, y);
+        x += y;
+        const double u = x + lane_move<kEight>(x);
         if ((l & 15) < QUADS) lds[threadIdx.x >> 6][k][quad * 4 + j] = u;
     }
     __syncthreads();
