@@ -733,8 +733,8 @@ int32_t pe_bn_bwd_bf16(const void* da, const void* a, int32_t relu, const void* 
  * Backward: from dh (may be NULL: 0) and dz (with pre) to dy, dx (may be NULL), dgate (with a
  * gate) and the parameter gradients asked for (overwritten, not added to).  dx may be dh, dy may
  * be dz, in place.  x and y are forward's inputs: h is rebuilt from them in float32.
- * workspace: pe_rnorm_bwd_workspace_bytes(d), 16-byte aligned, needed for parameter gradients
- * and for a gate shared by several rows.  The sums' order depends on the sizes alone.
+ * workspace: pe_rnorm_bwd_workspace_bytes(d) (0 for few rows), 16-byte aligned, needed for
+ * parameter gradients and for a gate shared by several rows.  The sums' order depends on the sizes alone.
  * ---------------------------------------------------------------------- */
 #define PE_RNORM_LAYER 0
 #define PE_RNORM_RMS   1

@@ -123,7 +123,7 @@ int32_t pe_tape_destroy(pe_tape_t tape) {
     return PE_OK;
 }
 
-int32_t pe_version(void) { return 1000; }
+int32_t pe_version(void) { return 1001; }
 
 const char* pe_last_error(void) { return pe::g_err; }
 

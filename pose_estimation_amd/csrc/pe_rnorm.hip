@@ -48,7 +48,8 @@ struct RnBwd {
     const void *dh, *dz, *y, *x, *gate;
     const float *stats, *gp, *bp, *s, *gq;
     void *dy, *dx, *dgate;
-    float* part;               // [items][slots][pitch]
+    float* part;               // [items][slots][pitch]; NULL: the only item writes the gradients
+    float *dgp, *dbp, *ds, *dgq, *dbq;
     int pitch, need;
     long rows, gate_rows;
     long lddh, lddz, ldy, ldx, ldg, lddy, lddx, lddg;
@@ -514,8 +515,8 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
         now = next;
     }
     if (!a.need) return;
-    const bool shared = !OWN && a.gate_rows;
-    float* out = a.part + (long)blockIdx.x * slots_of(a.gate_rows) * a.pitch;
+    const bool shared = !OWN && a.gate_rows, direct = a.part == nullptr;
+    float* out = direct ? nullptr : a.part + (long)blockIdx.x * slots_of(a.gate_rows) * a.pitch;
     if (in_wave(TEAM)) {
         // rows side by side in the wave, then the waves in order
 #pragma unroll
@@ -536,6 +537,7 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
         for (int c = threadIdx.x; c < a.C; c += kRnThreads) {
             float f = 1.0f, unused;
             if (shared) f = gate_value(as_float(static_cast<const YT*>(a.gate)[g * a.ldg + c]), a.act, unused);
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool weighted = a.need & (1 << i), plain = i >= 2 && (a.need & (4 << i));
@@ -543,10 +545,30 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
                     float v = fold[0][i][c];
 #pragma unroll
                     for (int wv = 1; wv < kRnThreads / 64; ++wv) v += fold[wv][i][c];
-                    if (weighted) out[(long)i * a.pitch + c] = i >= 2 ? v * f : v;
-                    if (plain) out[(long)(i + 2) * a.pitch + c] = v;
+                    sum[i] = v;
+                    if (weighted && !direct) out[(long)i * a.pitch + c] = i >= 2 ? v * f : v;
+                    if (plain && !direct) out[(long)(i + 2) * a.pitch + c] = v;
                 }
             }
+            if (direct) {
+                const float sc = a.s ? a.s[c] : 1.0f;
+                if (a.dgq) a.dgq[c] = sum[0];
+                if (a.dbq) a.dbq[c] = sum[1];
+                if (a.dgp) a.dgp[c] = sc * sum[2];
+                if (a.dbp) a.dbp[c] = sc * sum[3];
+                if (a.ds) a.ds[c] = (a.gp ? a.gp[c] : 1.0f) * sum[2] + (a.bp ? a.bp[c] * sum[3] : 0.0f);
+            }
+        }
+    } else if (direct) {
+        if (a.dgq) store8<MODE>(a.dgq, k, q1);
+        if (a.dbq) store8<MODE>(a.dbq, k, q0);
+        const f32x8 sc = load_param<MODE>(a.s, 1.0f, k);
+        if (a.dgp) store8<MODE>(a.dgp, k, sc * p1);
+        if (a.dbp) store8<MODE>(a.dbp, k, sc * p0);
+        if (a.ds) {
+            f32x8 v = load_param<MODE>(a.gp, 1.0f, k) * p1;
+            if (a.bp) v += load8<MODE>(a.bp, k) * p0;
+            store8<MODE>(a.ds, k, v);
         }
     } else {
         const f32x8 f = shared ? phi : splat(1.0f);
@@ -722,6 +744,7 @@ static long rows_at_once(int C) { return in_wave(team_of(C)) ? kRnThreads / team
 struct BwdGeom {
     long groups, group, nseg, rows_blk;
     long items() const { return groups * nseg; }
+    bool direct;   // one item, which writes the parameters' gradients: no fold, no workspace
 };
 
 static int pitch_of(int C) { return (C + 3) & ~3; }   // of a row of sums: 16-byte steps
@@ -738,7 +761,13 @@ static BwdGeom bwd_geom(const pe_rnorm_desc& d) {
     rows = (rows + at_once - 1) / at_once * at_once;
     if (rows < 1) rows = 1;
     g.rows_blk = rows;
-    g.nseg = (g.group + rows - 1) / rows;
+    // One workgroup and no fold while its rows cost less: 4 for each team inside a wave (32 x 256:
+    // 8.7 us; 33 rows by items and fold 9.0, and a launch more for the host), 2 for a workgroup
+    // (2 x 4096: 8.0, 4 rows 11.9; 5 rows by items 8.4), 1 past 4096 channels.
+    const int team = team_of(d.C);
+    g.direct = !grouped && d.rows <= (in_wave(team) ? 4 * at_once : team == 512 ? 2 : 1);
+    if (g.direct) g.rows_blk = d.rows;
+    g.nseg = (g.group + g.rows_blk - 1) / g.rows_blk;
     return g;
 }
 
@@ -869,8 +898,8 @@ extern "C" int32_t pe_rnorm_fwd(const pe_rnorm_desc* d, const void* y, const voi
                "pe_rnorm_fwd: output rows overlap");
     PE_REQUIRE(!d->pre || z, PE_E_INVALID, "pe_rnorm_fwd: NULL z");
     PE_REQUIRE(d->gate_rows == 0 || gate, PE_E_INVALID, "pe_rnorm_fwd: NULL gate");
-    PE_REQUIRE(d->post || !(post_gamma || post_beta), PE_E_INVALID,
-               "pe_rnorm_fwd: parameters of a norm that is off");
+    PE_REQUIRE((d->post || !(post_gamma || post_beta)) && (d->pre || !(pre_gamma || pre_beta || z)),
+               PE_E_INVALID, "pe_rnorm_fwd: operands of a norm that is off");
     PE_REQUIRE(element_aligned(d->y_dtype, {y, gate, z}) && element_aligned(d->x_dtype, {x, h}) &&
                    element_aligned(PE_DTYPE_F32, {post_gamma, post_beta, scale, pre_gamma, pre_beta, stats}),
                PE_E_INVALID, "pe_rnorm_fwd: a pointer between two elements");
@@ -936,7 +965,9 @@ extern "C" int32_t pe_rnorm_fwd(const pe_rnorm_desc* d, const void* y, const voi
 extern "C" size_t pe_rnorm_bwd_workspace_bytes(const pe_rnorm_desc* d) {
     if (pe::check_desc("pe_rnorm_bwd_workspace_bytes", d) != PE_OK) return 0;
     if (d->rows == 0) return 0;
-    const long items = pe::bwd_geom(*d).items();
+    const pe::BwdGeom g = pe::bwd_geom(*d);
+    if (g.direct) return 0;
+    const long items = g.items();
     const long slices = items > pe::kFoldItems ? pe::kFoldSlices : 0;
     return sizeof(float) * (size_t)pe::pitch_of(d->C) *
            (size_t)(items * pe::slots_of(d->gate_rows) + 4 * slices);
@@ -953,12 +984,9 @@ extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const vo
     using namespace pe;
     const int32_t bad = check_desc("pe_rnorm_bwd", d);
     if (bad) return bad;
-    PE_REQUIRE(d->post || !(post_gamma || post_beta), PE_E_INVALID,
-               "pe_rnorm_bwd: parameters of a norm that is off");
-    PE_REQUIRE(d->post || !(dpost_gamma || dpost_beta), PE_E_INVALID,
-               "pe_rnorm_bwd: gradients of a norm that is off");
-    PE_REQUIRE(d->pre || !(dpre_gamma || dpre_beta || dz), PE_E_INVALID,
-               "pe_rnorm_bwd: gradients of a norm that is off");
+    PE_REQUIRE((d->post || !(post_gamma || post_beta || dpost_gamma || dpost_beta)) &&
+                   (d->pre || !(pre_gamma || dpre_gamma || dpre_beta || dz)),
+               PE_E_INVALID, "pe_rnorm_bwd: operands of a norm that is off");
     PE_REQUIRE(element_aligned(d->y_dtype, {dz, y, gate, dy, dgate}) &&
                    element_aligned(d->x_dtype, {dh, x, dx}) &&
                    element_aligned(PE_DTYPE_F32, {stats, post_gamma, post_beta, scale, pre_gamma, dpost_gamma,
@@ -969,7 +997,7 @@ extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const vo
     const int need = (dpre_gamma ? kQ1 : 0) | (dpre_beta ? kQ0 : 0) | (dpost_gamma || dscale ? kP1 : 0) |
                      (dpost_beta || (dscale && post_beta) ? kP0 : 0) | (grouped ? kG1 : 0) |
                      (grouped && post_beta ? kG0 : 0);
-    BwdGeom g{0, 0, 0, 0};
+    BwdGeom g{0, 0, 0, 0, false};
     if (d->rows) {
         PE_REQUIRE(y && dy, PE_E_INVALID, "pe_rnorm_bwd: NULL y or dy");
         PE_REQUIRE(dh || dz, PE_E_INVALID, "pe_rnorm_bwd: neither dh nor dz");
@@ -982,7 +1010,7 @@ extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const vo
                    "pe_rnorm_bwd: rows of dgate overlap");
         g = bwd_geom(*d);
         PE_REQUIRE(g.items() <= 0x7fffffffl, PE_E_UNSUPPORTED, "pe_rnorm_bwd: too many gate rows");
-        if (need) {
+        if (need && !g.direct) {
             PE_REQUIRE(workspace && aligned(workspace, 16), PE_E_INVALID,
                        "pe_rnorm_bwd: workspace must be given, 16-byte aligned");
             PE_REQUIRE(workspace_bytes >= pe_rnorm_bwd_workspace_bytes(d), PE_E_INVALID,
@@ -1003,7 +1031,12 @@ extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const vo
         a.dy = dy;
         a.dx = dx;
         a.dgate = dgate;
-        a.part = static_cast<float*>(workspace);
+        a.part = g.direct ? nullptr : static_cast<float*>(workspace);
+        a.dgp = dpost_gamma;
+        a.dbp = dpost_beta;
+        a.ds = dscale;
+        a.dgq = dpre_gamma;
+        a.dbq = dpre_beta;
         a.pitch = pitch_of(d->C);
         a.need = need;
         a.rows = d->rows;
@@ -1035,7 +1068,7 @@ extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const vo
             launch_bwd<uint16_t, uint16_t>(a, items, as_stream(stream));
         }
     }
-    if (!sums && !(grouped && d->rows)) return check_launch("pe_rnorm_bwd");
+    if (g.direct || (!sums && !(grouped && d->rows))) return check_launch("pe_rnorm_bwd");
     RnFold f{};
     f.part = static_cast<float*>(workspace);
     f.gp = post_gamma;

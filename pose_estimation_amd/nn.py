@@ -20,6 +20,7 @@ from ._ffi import (PE_CONV_MAX_CHAIN, PE_DTYPE_BF16, PE_DTYPE_F32, PE_GATE_NONE,
 from .ops import _need_gpu, _ptr, _stream, on_device
 
 BF16 = torch.bfloat16
+F32 = torch.float32
 
 
 # --------------------------------------------------------------------------- packers
@@ -1341,8 +1342,7 @@ def _row_stride(t: torch.Tensor, name: str) -> int:
 def _channel_vector(t: Optional[torch.Tensor], C: int, index: int, name: str):
     if t is None:
         return None
-    if t.dtype is not torch.float32 or t.dim() != 1 or t.numel() != C or not t.is_contiguous() or \
-            t.get_device() != index:
+    if t.dtype is not F32 or t.shape != (C,) or not t.is_contiguous() or t.get_device() != index:
         raise ValueError(f"{name} must be contiguous float32 [{C}] on the device of y")
     return t.data_ptr()
 
@@ -1520,17 +1520,22 @@ def residual_norm_bwd(dh: Optional[torch.Tensor], dz: Optional[torch.Tensor], y:
         into = {k: o for k, o in into.items() if o is not None}
         if not into.keys() <= set(want):
             raise ValueError(f"no such parameter gradients: {sorted(into.keys() - set(want))}")
-        if len({_channel_vector(o, C, index, k) for k, o in into.items()}) < len(into):
+        at = sorted(_channel_vector(o, C, index, k) for k, o in into.items())
+        if any(b - a < 4 * C for a, b in zip(at, at[1:])):
             raise ValueError("two parameter gradients share memory")
         grads.update(into)
         want = [k for k in want if k not in into]
     if want:
         grads.update(zip(want, y.new_empty((len(want), C), dtype=torch.float32).unbind(0)))
+    nbytes = 0
     if workspace is None:
-        workspace = y.new_empty(lib().pe_rnorm_bwd_workspace_bytes(ctypes.addressof(d)),
-                                dtype=torch.uint8)
+        nbytes = lib().pe_rnorm_bwd_workspace_bytes(ctypes.addressof(d))
+        if nbytes:
+            workspace = y.new_empty(nbytes, dtype=torch.uint8)
     elif workspace.device != y.device or not workspace.is_contiguous():
         raise ValueError(f"workspace must be contiguous on {y.device}")
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
     if dgate is not None and rows == 0:
         dgate.zero_()
     with on_device(y):
@@ -1538,8 +1543,8 @@ def residual_norm_bwd(dh: Optional[torch.Tensor], dz: Optional[torch.Tensor], y:
             ctypes.addressof(d), _ptr(dh), _ptr(dz), y.data_ptr(), _ptr(x), _ptr(stats), gp, bp,
             scale, _ptr(gate), gq, dy.data_ptr(), _ptr(dx), _ptr(dgate),
             _ptr(grads["dpost_gamma"]), _ptr(grads["dpost_beta"]), _ptr(grads["dscale"]),
-            _ptr(grads["dpre_gamma"]), _ptr(grads["dpre_beta"]), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _stream(y)))
+            _ptr(grads["dpre_gamma"]), _ptr(grads["dpre_beta"]), _ptr(workspace), nbytes,
+            _stream(y)))
     return {"dy": dy, "dx": dx, "dgate": dgate, **grads}
 
 

@@ -461,7 +461,8 @@ class GradSet:
     strides (the gradient itself allowed); None: in place.
 
     The set keeps the tensors and reads their values anew at every call, so a program builds it
-    once over the gradients that every step refills in place.  Tensors that share memory with
+    once over the gradients that every step refills in place.  It can be used on any stream of
+    its device, by several at a time, and in a captured graph, which it has to outlive.  Tensors that share memory with
     one another are refused: they would count twice, and be scaled twice."""
 
     _SPAN = np.dtype([("src", np.uint64), ("dst", np.uint64), ("n", np.int64),

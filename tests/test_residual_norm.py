@@ -264,7 +264,7 @@ def test_forward_refuses(on_cpu):
 
 def test_backward_refuses(on_cpu):
     y, v = torch.zeros(6, 16), torch.zeros(16)
-    stats, on = torch.zeros(4, 6), (v, None)
+    stats, on, wide = torch.zeros(4, 6), (v, None), torch.zeros(40)
     for args, kw in (
             ((None, None, y, y, None), {}), ((y, y, y, y, None), {}), ((y, None, y, y, stats), dict(pre=on)),
             ((y, None, y, y, None), dict(post=on)), ((y, None, y, y, stats[:, :5]), dict(post=on)),
@@ -276,7 +276,9 @@ def test_backward_refuses(on_cpu):
             ((y, None, y, y, stats), dict(post=on, into={"dpost_beta": v})),
             ((y, None, y, y, stats), dict(post=on, into={"dnothing": v})),
             ((y, None, y, y, stats), dict(post=on, into={"dpost_gamma": torch.zeros(15)})),
-            ((y, None, y, y, stats), dict(post=(v, v), into={"dpost_gamma": v, "dpost_beta": v}))):
+            ((y, None, y, y, stats), dict(post=(v, v), into={"dpost_gamma": v, "dpost_beta": v})),
+            ((y, None, y, y, stats), dict(post=(v, v), into={"dpost_gamma": wide[:16],
+                                                             "dpost_beta": wide[15:31]}))):
         with pytest.raises(ValueError):
             nn.residual_norm_bwd(*args, **kw)
 
@@ -321,11 +323,13 @@ def test_c_entries_refuse_bad_descriptions():
         assert lib.pe_rnorm_bwd_workspace_bytes(ctypes.addressof(d)) == 0
     assert fwd(desc(), y=None) == E and fwd(desc(), h=None) == E and fwd(desc(), z=None) == E
     assert fwd(desc(post=0)) == E and fwd(desc(gate_rows=3)) == E and fwd(desc(ldh=8)) == E
+    assert fwd(desc(pre=0)) == E and fwd(desc(), x=17) == E and bwd(desc(), dh=17) == E
     assert bwd(desc(), dh=None, dz=None) == E and bwd(desc(), dz=None) == E
     assert bwd(desc(), stats=None) == E and bwd(desc(), dy=None) == E and bwd(desc(lddy=8)) == E
     assert bwd(desc(gate_rows=3), gate=one) == E and bwd(desc(gate_rows=3), dgate=one) == E
     assert bwd(desc(post=0)) == E and bwd(desc(pre=0), dgq=one) == E
-    assert bwd(desc(), ws=None) == E and bwd(desc(), ws=8) == E and bwd(desc(), n=10) == E
+    many = desc(rows=6000)
+    assert bwd(many, ws=None) == E and bwd(many, ws=8) == E and bwd(many, n=10) == E
     assert fwd(desc(rows=0)) == 0
     need = lib.pe_rnorm_bwd_workspace_bytes
     for rows, C, per in itertools.product((1, 7, 1000, 200_000), (1, 64, 333, 8192), (0, 1, 2)):
@@ -333,7 +337,8 @@ def test_c_entries_refuse_bad_descriptions():
             d = desc(rows=rows, C=C, gate_rows=per)
             n = need(ctypes.addressof(d))
             items = max(1100, rows // 2) if per == 2 else 1100
-            assert 16 * C <= n <= 24 * (C + 3) * (items + 64)
+            assert n <= 24 * (C + 3) * (items + 64)
+            assert n >= 16 * C or (rows <= 7 and per != 2)   # one workgroup needs none
 
 
 def test_the_expected_values_are_those_of_automatic_differentiation():
@@ -399,7 +404,7 @@ def test_every_width_against_float64(types, norm, C):
 
 
 @gpu
-@pytest.mark.parametrize("rows", [1, 2, 31, 33, 257, 1025, 5000])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 31, 32, 33, 257, 1025, 5000])
 @pytest.mark.parametrize("C", [24, 256, 1032])
 def test_row_counts(rows, C):
     check(make(rows, C, "mixed"), "layer")
