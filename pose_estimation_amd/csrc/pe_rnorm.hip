@@ -24,7 +24,9 @@ constexpr int kRnEl = 8;          // channels a thread holds
 constexpr int kRnThreads = 256;   // of a workgroup whose rows are shorter than a wave's reach
 // Items of backward (workgroups, each with a set of partial sums), about.  Two a CU: at 196608 x
 // 256 bf16 the launch takes 141, 129, 133, 145, 138 us with 256, 512, 768, 1024, 2048 of them, at
-// 3456 x 2048 29, 26, 28, 30, 35 us, and the fold behind it grows with their number.
+// 3456 x 2048 29, 26, 28, 30, 35 us, and the fold behind it grows with their number.  More where a
+// row takes a workgroup of less than 256 threads, for as many threads in all (16000 x 1024: both
+// launches 55 us, with 512 items 68), as long as an item has eight rows (2000 x 1024: 23 us, 26).
 constexpr int kRnItems = 512;
 // The sums an item leaves, as bits of what anything needs: of dz*hhat, dz, D*phi*yhat and D*phi,
 // and with a gate shared by several rows also of D*yhat and D.
@@ -425,7 +427,9 @@ struct RnRow {
 };
 
 // OWN: a gate row for each row.  The next row is loaded while this one is worked on.  Workgroups
-// of more than 512 threads, which have 128 registers a thread, keep the parameters in LDS.
+// of more than 512 threads have 128 registers a thread: they keep the parameters in LDS and load
+// no row ahead (4000 x 8192 bf16: 117 us; with the parameters in registers 127, with the row
+// ahead and spilled registers 137, with a gate per row 177 against 253).
 template <typename YT, typename XT, bool OWN, int TEAM, int MODE>
 __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_kernel(RnBwd a) {
     __shared__ double2 lds[in_wave(TEAM) ? 1 : 32];
@@ -466,9 +470,11 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
     f32x8 q1 = splat(0.0f), q0 = q1, p1 = q1, p0 = q1;
     long row = lo + (in_wave(TEAM) ? (int)threadIdx.x / T : 0);
     RnRow<YT, XT, OWN, MODE> now, next;
-    if (row < hi) now.load(a, row, k);
+    constexpr bool AHEAD = !WIDE;
+    if (AHEAD && row < hi) now.load(a, row, k);
     for (; row < hi; row += teams) {
-        if (row + teams < hi) next.load(a, row + teams, k);
+        if (!AHEAD) now.load(a, row, k);
+        if (AHEAD && row + teams < hi) next.load(a, row + teams, k);
         f32x8 y = now.y.value(), d = now.dh.value();
         if (OWN) gate8(now.gate.value(), a.act, phi, slope);
         if (a.post) y = (y - now.py) * now.ry;
@@ -512,7 +518,7 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
             w = fma8(y, splat(-n2), w - n1) * now.ry;
         }
         store8<MODE>(static_cast<YT*>(a.dy) + row * a.lddy, k, w);
-        now = next;
+        if (AHEAD) now = next;
     }
     if (!a.need) return;
     const bool shared = !OWN && a.gate_rows, direct = a.part == nullptr;
@@ -756,7 +762,10 @@ static BwdGeom bwd_geom(const pe_rnorm_desc& d) {
     g.group = grouped ? d.gate_rows : d.rows;
     g.groups = grouped ? d.rows / d.gate_rows : 1;
     const long at_once = rows_at_once(d.C);
-    long want = (kRnItems + g.groups - 1) / g.groups;
+    long want = kRnItems * 256 / (long)block_of(d.C);
+    if (want > d.rows / 8) want = d.rows / 8;
+    if (want < kRnItems) want = kRnItems;
+    want = (want + g.groups - 1) / g.groups;
     long rows = (g.group + want - 1) / want;
     rows = (rows + at_once - 1) / at_once * at_once;
     if (rows < 1) rows = 1;
