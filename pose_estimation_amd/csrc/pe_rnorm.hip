@@ -8,8 +8,13 @@
 // it from its load to its store, so statistics, both norms and the gate cost no further pass.
 // Eight channels a thread (one 16-byte load of bf16): a team is the next power of two of C/8
 // threads inside one wave (1 to 64, several rows a wave side by side), or, past 512 channels, a
-// workgroup of its own.  Means and variances are taken in two steps from the registers (no
-// difference of large sums), all arithmetic is float32, each output is rounded once.
+// workgroup of its own.  Means and variances come from the registers, in two steps or from float64
+// sums (no difference of large float32 sums); all other arithmetic is float32, each output is
+// rounded once.  Wider shares of a row per thread would not leave a wave the registers to have
+// the next row under way, narrower ones add lanes to every sum.
+// Measured: forward 8192 x 4096 bf16 with a float32 residual and a gate per row 92 us (5.1 TB/s),
+// 196608 x 256 bf16 82 us (4.9 TB/s) and backward there 131 us (4.6 TB/s; a copy reaches 4.7),
+// one row of 4096 3.4 us.
 #include <math.h>
 
 #include <initializer_list>
@@ -399,8 +404,8 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_k
 // as reading the stored h, without its rounding in the gradients.  Four sums a channel stay in
 // registers over an item's rows and go to the workspace once an item; a second launch folds the
 // items in order in float64, so the results have the same bits on every call.  An item never
-// crosses a gate row: phi is a constant of the item and is left out of its sums (the fold knows
-// the item's gate), unless the gate has a row for each row, whose gradient needs no sum.
+// crosses a gate row: phi is a constant of the item, which leaves its sums of D with phi (for the
+// parameters) and without (for the gate).  A gate row for each row has its gradient in the loop.
 template <typename YT, typename XT, bool OWN, int MODE>
 struct RnRow {
     Raw<YT, MODE> y, dz, gate;
