@@ -259,7 +259,8 @@ int32_t pe_sgd_step(float* p, float* mom, const float* grad, uint16_t* p_bf16,
  * gradient overflows or vanishes; *norm is the float32 value of n.  max_norm may be +inf (never
  * clips) and 0 (all zero).  If any gradient is NaN or infinite so is n, and every clipped value
  * is NaN; with skip_nonfinite an optimizer step then changes nothing but *norm.
- * The order of the sums depends on the lengths alone: the same gradients give the same bits.
+ * The order of the sums depends on the lengths and 16-byte alignment alone: the same gradients in
+ * the same layout give the same bits.
  *
  * A set of tensors is a DEVICE table of contiguous spans, cut into shares: a wave handles spans
  * [begin[i], begin[i+1]) (begin: DEVICE array of shares + 1 entries, shares <= PE_NORM_MAX_SHARES),

@@ -10,7 +10,8 @@
 // waits for another, none has a long list to walk, and there is no search for the tensor an
 // element is in.  Squares are summed in float64: float32 squares overflow from 1.8e19 on and
 // vanish below 1e-23, and the conversion is hidden behind the loads.  The sums' order depends
-// only on the lengths, so the result has the same bits on every call and every rank.
+// only on the tensors' lengths and 16-byte alignment, so the result has the same bits on every
+// call, and on every rank with the same layout.
 // Measured, 34 M float32 gradients in 170 tensors: the norm 26 us (5.2 TB/s; a share per workgroup
 // of 256 threads with one load a lane under way: 27 and, out of cold caches, 41), the clipping of
 // them into other tensors 47 us more; nine small tensors 4.5 us in one launch (5.5 in two).

@@ -657,7 +657,8 @@ class TrainGraph:
                        clip_norm: Optional[float] = None, skip_nonfinite: bool = False) -> None:
         """clip_norm: limit of the gradients' global norm, taken after the exchange, so that every
         rank clips alike; self.grad_norm is then the norm before clipping ([1], on the device).
-        skip_nonfinite: leave everything as it is when that norm is not finite."""
+        skip_nonfinite: leave parameters and moments as they are when that norm is not
+        finite (the step still counts, and running statistics have moved in its forward pass)."""
         scale = 1.0
         if self.bucketer is not None:
             self.bucketer.finish()

@@ -351,7 +351,8 @@ def adam_step(p: torch.Tensor, m: torch.Tensor, v: torch.Tensor, grad: torch.Ten
     leaves `grad` as it is, and return the norm before clipping, [1] float32 on the device.
     The norm is taken over `grad`, or over `norm_over`, a GradSet, where the arena is only a
     part of what is clipped together.  A norm that is not finite makes every parameter NaN, or
-    with skip_nonfinite leaves p, m, v and p_bf16 untouched; max_norm = inf only skips."""
+    with skip_nonfinite leaves p, m, v and p_bf16 untouched (`step` is the caller's count);
+    max_norm = inf only skips."""
     _need_gpu(p, m, v, grad, p_bf16)
     for t in (p, m, v, grad):
         if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != p.numel():
@@ -462,7 +463,8 @@ class GradSet:
 
     The set keeps the tensors and reads their values anew at every call, so a program builds it
     once over the gradients that every step refills in place.  It can be used on any stream of
-    its device, by several at a time, and in a captured graph, which it has to outlive.  Tensors that share memory with
+    its device, by several at a time, and in a captured graph, which it has to outlive.  The
+    tensors must stay in place: not resized, not given other memory.  Tensors that share memory with
     one another are refused: they would count twice, and be scaled twice."""
 
     _SPAN = np.dtype([("src", np.uint64), ("dst", np.uint64), ("n", np.int64),

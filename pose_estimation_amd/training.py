@@ -518,7 +518,8 @@ class TrainablePoseResNet(PoseResNet):
         the forward/loss/backward pass from the call list recorded on the first step.
         clip_norm: limit of the gradients' global norm, taken after the exchange, so that every
         rank clips alike; self.grad_norm is then the norm before clipping ([1], on the device).
-        skip_nonfinite: leave parameters and moments as they are when that norm is not finite.
+        skip_nonfinite: leave parameters and moments as they are when that norm is not finite
+        (the step still counts, and running statistics have moved in its forward pass).
         Returns (loss [1] float32 device tensor, per_joint [K])."""
         if host_replay:
             loss, per_joint = self.replay_host(self._pass, images_u8, x_s2d, joints, mask)

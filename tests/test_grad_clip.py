@@ -430,6 +430,60 @@ def test_captured_calls_and_other_streams_give_the_eager_bits():
 
 
 @gpu
+def test_given_norm_and_workspace_are_used():
+    g = rand(seeded(6), 300_000)
+    out, ws = torch.zeros(1, device="cuda"), torch.zeros(ops._NORM_WS + 8, dtype=torch.uint8, device="cuda")
+    s = pe.GradSet(g)
+    want = pe.grad_norm(s)
+    assert pe.grad_norm(s, out=out, workspace=ws) is out and torch.equal(out, want)
+    assert bool(ws.any())
+    out.zero_()
+    assert pe.clip_grads(s, INF, out=out, workspace=ws) is out and torch.equal(out, want)
+    p, m, v, grad, _ = arenas(50_000, 5)
+    pe.adam_step(p, m, v, grad, 1, max_norm=1.0, workspace=ws)
+    with pytest.raises(_ffi.PeError):                     # between two float64
+        pe.grad_norm(s, workspace=ws[4:])
+
+
+@gpu
+def test_tensors_past_four_gigabytes():
+    """Offsets that do not fit 32 bits, in a set and in the arenas of a step."""
+    n = (1 << 31) + 5
+    g = torch.zeros(n, device="cuda")
+    at = torch.tensor([0, 1, n // 2, n - 2, n - 1], device="cuda")
+    g[at] = torch.tensor([3.0, -1.0, 2.0, 5.0, -4.0], device="cuda")
+    want = math.sqrt(55.0)
+    assert_norm(pe.grad_norm([g]), want)
+    assert_norm(pe.clip_grads(pe.GradSet(g[3:]), 0.5 * math.sqrt(45.0)), math.sqrt(45.0))
+    assert g[at].tolist() == [3.0, -1.0, 1.0, 2.5, -2.0]
+    p, mom = torch.ones(n, device="cuda"), torch.zeros(n, device="cuda")
+    norm = pe.sgd_step(p, mom, g, 0.5, max_norm=1e9)
+    assert_norm(norm, math.sqrt(9.0 + 1.0 + 1.0 + 6.25 + 4.0))
+    assert p[at].tolist() == [-0.5, 1.5, 0.5, -0.25, 2.0] and float(p[n // 2 + 1]) == 1.0
+    assert int((p != 1.0).sum()) == 5
+
+
+@gpu
+def test_a_recorded_call_list_repeats_the_calls():
+    from pose_estimation_amd import replay
+
+    g, out = rand(seeded(3), 70_001), torch.empty(70_001, device="cuda")
+    s = pe.GradSet([g], out=[out])
+
+    def work(x):
+        g.copy_(x)
+        return pe.grad_norm(s), pe.clip_grads(s, 1.0)
+
+    rec = replay.RecordedPass(work, [rand(seeded(4), 70_001)], g.device)
+    for seed in (5, 6):
+        x = rand(seeded(seed), 70_001)
+        got = [t.clone() for t in rec(x)] + [out.clone()]
+        want = list(work(x)) + [out]
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@gpu
 @pytest.mark.parametrize("optimizer", ["adam", "sgd"])
 def test_trainer_clips_as_configured(optimizer):
     """A trainer step with the limit equals the same step on gradients clipped beforehand, and a
