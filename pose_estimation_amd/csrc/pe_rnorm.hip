@@ -15,6 +15,7 @@
 // Measured: forward 8192 x 4096 bf16 with a float32 residual and a gate per row 92 us (5.1 TB/s),
 // 196608 x 256 bf16 82 us (4.9 TB/s) and backward there 131 us (4.6 TB/s; a copy reaches 4.7),
 // one row of 4096 3.4 us.
+#include <float.h>
 #include <math.h>
 
 #include <initializer_list>
@@ -46,7 +47,6 @@ struct RnFwd {
     long rows, gate_rows;      // rows per gate row; 0 = no gate
     long ldy, ldx, ldg, ldh, ldz;
     long rows_blk;
-    double inv_c64;
     float eps, inv_c;
     int C, post, pre, layer, act;
 };
@@ -79,9 +79,10 @@ __device__ __forceinline__ int team_size() {
 
 // How a row's channels lie over its threads.  WHOLE (C a multiple of 8): thread t has channels 8t
 // to 8t+7.  TAIL: the last thread has the row's last eight, which the one before it shares: it
-// computes them all and counts and stores only those from `first` on, so that no load needs a
-// branch of its own (which would make the wave wait for it).  FEW (C < 8): one channel a thread.
-// Rows start at any element: 16-byte accesses need no alignment here.
+// computes them all and counts and stores only those from `first` on.  FEW (C < 8): one channel a
+// thread.  Threads past the row read its last channels and count nothing, so that no load needs a
+// branch of its own (which would make the wave wait for it).  Rows start at any element: 16-byte
+// accesses need no alignment here.
 enum { WHOLE, TAIL, FEW };
 
 template <int MODE>
@@ -89,13 +90,10 @@ struct Cols {
     int c, first;
     bool on;
     __device__ __forceinline__ Cols(int t, int C) {
-        on = t * (MODE == FEW ? 1 : kRnEl) < C;
-        c = MODE == FEW ? t : t * kRnEl;
-        first = 0;
-        if (MODE == TAIL && c > C - kRnEl) {
-            first = c - (C - kRnEl);
-            c = C - kRnEl;
-        }
+        constexpr int N = MODE == FEW ? 1 : kRnEl;
+        on = t * N < C;
+        c = t * N < C - N ? t * N : C - N;
+        first = t * N - c;
     }
     // Whether the thread's j-th value is a channel of its own.
     __device__ __forceinline__ bool mine(int j) const {
@@ -113,7 +111,7 @@ typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 // A row's channels as they come from memory, so that the next row can be on its way in few
-// registers while this one is worked on.  Threads without channels read as 0.
+// registers while this one is worked on.
 template <typename T, int MODE>
 struct Raw;
 
@@ -122,7 +120,7 @@ struct Raw<float, MODE> {
     f32x4 a, b;
     __device__ __forceinline__ void load(const float* p, const Cols<MODE>& k, bool use = true) {
         a = b = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (use && k.on) {
+        if (use) {
             if (MODE == FEW) {
                 a.x = p[k.c];
             } else {
@@ -141,7 +139,7 @@ struct Raw<uint16_t, MODE> {
     u32x4 v;
     __device__ __forceinline__ void load(const uint16_t* p, const Cols<MODE>& k, bool use = true) {
         v = u32x4{0, 0, 0, 0};
-        if (use && k.on) {
+        if (use) {
             if (MODE == FEW) {
                 v.x = p[k.c];
             } else {
@@ -198,41 +196,49 @@ __device__ __forceinline__ f32x8 load_param(const float* p, float absent, const 
     return p ? load8<MODE>(p, k) : splat(absent);
 }
 
-__device__ __forceinline__ float sum8(f32x8 v) {
-    return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-}
-
-// 0 in the place of channels that are not the thread's own.
+// A thread's share of a sum over the row, and of a sum of squares.
 template <int MODE>
-__device__ __forceinline__ f32x8 inside(f32x8 v, const Cols<MODE>& k) {
+__device__ __forceinline__ f32x8 own(f32x8 v, const Cols<MODE>& k) {
+    if (MODE == WHOLE) return v;
 #pragma unroll
     for (int j = 0; j < kRnEl; ++j) v[j] = k.mine(j) ? v[j] : 0.0f;
     return v;
 }
 
+template <int MODE>
+__device__ __forceinline__ float own_sum(f32x8 v, const Cols<MODE>& k) {
+    v = own<MODE>(v, k);
+    const float s = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    return MODE != WHOLE || k.on ? s : 0.0f;
+}
+
+template <int MODE>
+__device__ __forceinline__ float own_squares(f32x8 v, const Cols<MODE>& k) {
+    v = own<MODE>(v, k);
+    const f32x4 q = __builtin_elementwise_fma(v.hi, v.hi, v.lo * v.lo);
+    const float s = (q[0] + q[1]) + (q[2] + q[3]);
+    return MODE != WHOLE || k.on ? s : 0.0f;
+}
+
 // ---- sums over a row's team ---------------------------------------------------------------
-// A workgroup as a team: the waves' sums through LDS in order; two buffers in turn, so one
-// barrier a sum is enough.
+// A workgroup as a team: the waves' values through LDS, then a lane for each of the at most 16
+// waves (with a loop over them instead 4000 x 8192 bf16 took 77 us, not 69); two buffers in turn, so
+// one barrier a sum is enough.
 struct TeamSums {
-    double2* buf;   // LDS [2][16], workgroup teams only
+    float2* buf;    // LDS [2][16], workgroup teams only
     int turn;
-    double inv_c;   // 1 / C, forward only
+    // 1 / this wave's channels, and the channels of the wave of the lane's index; forward only
+    float per_wave, in_lane;
 };
 
-template <typename T2, typename T>
-__device__ __forceinline__ void waves_sum2(T& a, T& b, TeamSums& ts) {
-    T2* buf = reinterpret_cast<T2*>(ts.buf + 16 * ts.turn);
+__device__ __forceinline__ float2 each_wave(float2 v, TeamSums& ts) {
+    float2* buf = ts.buf + 16 * ts.turn;
     ts.turn ^= 1;
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = T2{a, b};
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
     __syncthreads();
-    const int waves = (int)blockDim.x >> 6;
-    T2 v = buf[0];
-    for (int i = 1; i < waves; ++i) {
-        v.x += buf[i].x;
-        v.y += buf[i].y;
-    }
-    a = v.x;
-    b = v.y;
+    const int w = (int)threadIdx.x & 15;
+    v = buf[w];
+    return w < (int)blockDim.x >> 6 ? v : float2{0.0f, 0.0f};
 }
 
 template <int TEAM>
@@ -240,53 +246,42 @@ __device__ __forceinline__ void team_sum2(float& a, float& b, TeamSums& ts) {
     constexpr int W = in_wave(TEAM) ? TEAM : 64;
     a = lanes_sum<W>(a);
     b = lanes_sum<W>(b);
-    if (!in_wave(TEAM)) waves_sum2<float2>(a, b, ts);
+    if (!in_wave(TEAM)) {
+        const float2 v = each_wave(float2{a, b}, ts);
+        a = lanes_sum<16>(v.x);
+        b = lanes_sum<16>(v.y);
+    }
 }
 
-template <int TEAM>
-__device__ __forceinline__ float team_sum(float a, TeamSums& ts) {
-    a = lanes_sum<in_wave(TEAM) ? TEAM : 64>(a);
-    float unused = 0.0f;
-    if (!in_wave(TEAM)) waves_sum2<float2>(a, unused, ts);
-    return a;
-}
-
-// mean and rstd of the row, v replaced by the normalised row.  Inside a wave mean and variance
-// are taken one after the other.  A workgroup would pay a barrier for each: it sums values and
-// squares together in float64, where the squares of float32 are exact and their difference
-// from the mean's square is good to 2^-53 of the larger.
+// mean and rstd of the row, v replaced by the normalised row.  In two steps, the second about the
+// first's mean, so that no large sums cancel.  A workgroup would pay a barrier for each step: its
+// waves take both about their own means m_w and are joined behind one,
+//   sum (v - m)^2 = sum_w (sum (v - m_w)^2 + n_w (m_w - m)^2).
 template <int TEAM, int MODE>
 __device__ __forceinline__ void normalise(f32x8& v, const Cols<MODE>& k, float inv_c, float eps,
                                           bool layer, float& mean, float& rstd, TeamSums& ts) {
+    constexpr int W = in_wave(TEAM) ? TEAM : 64;
     mean = 0.0f;
-    float var;
-    if (layer && !in_wave(TEAM)) {
-        const f32x8 in = inside<MODE>(v, k);
-        double s1 = 0.0, s2 = 0.0;
-#pragma unroll
-        for (int j = 0; j < kRnEl; ++j) {
-            const double x = (double)in[j];
-            s1 += x;
-            s2 = __builtin_fma(x, x, s2);
-        }
-        s1 = lanes_sum<64>(s1);
-        s2 = lanes_sum<64>(s2);
-        waves_sum2<double2>(s1, s2, ts);
-        const double m = s1 * ts.inv_c;
-        mean = (float)m;
-        var = (float)__builtin_fma(-m, m, s2 * ts.inv_c);
-        if (var < 0.0f) var = 0.0f;   // NaN stays
-        v -= mean;
-    } else {
-        if (layer) {
-            mean = team_sum<TEAM>(sum8(inside<MODE>(v, k)), ts) * inv_c;
-            v -= mean;
-        }
-        const f32x8 in = inside<MODE>(v, k);
-        var = team_sum<TEAM>(sum8(in * in), ts) * inv_c;
+    f32x8 c = v;
+    if (layer) {
+        mean = lanes_sum<W>(own_sum<MODE>(v, k)) * (in_wave(TEAM) ? inv_c : ts.per_wave);
+        c = v - mean;
     }
-    rstd = 1.0f / sqrtf(var + eps);
-    v *= rstd;
+    float var = lanes_sum<W>(own_squares<MODE>(c, k)), shift = 0.0f;
+    if (!in_wave(TEAM)) {
+        const float own_mean = mean;
+        const float2 w = each_wave(float2{mean, var}, ts);
+        if (layer) {
+            mean = lanes_sum<16>(w.x * ts.in_lane) * inv_c;
+            const float d = w.x - mean;
+            var = lanes_sum<16>(__builtin_fmaf(d * ts.in_lane, d, w.y));
+            shift = own_mean - mean;
+        } else {
+            var = lanes_sum<16>(w.y);
+        }
+    }
+    rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(var, inv_c, eps));   // good to 2^-23; eps is normal
+    v = in_wave(TEAM) ? c * rstd : fma8(c, splat(rstd), splat(shift * rstd));
 }
 
 // ---- gate ---------------------------------------------------------------------------------
@@ -343,12 +338,20 @@ struct FwdRow {
 
 template <typename YT, typename XT, bool OWN, int TEAM, int MODE>
 __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_kernel(RnFwd a) {
-    __shared__ double2 lds[in_wave(TEAM) ? 1 : 32];
-    TeamSums ts{lds, 0, a.inv_c64};
+    __shared__ float2 lds[in_wave(TEAM) ? 1 : 32];
     const int T = team_size<TEAM>();
     const int t = in_wave(TEAM) ? (int)threadIdx.x % T : (int)threadIdx.x;
     const int teams = in_wave(TEAM) ? kRnThreads / T : 1;
     const Cols<MODE> k(t, a.C);
+    auto channels_of = [&](int wave) {
+        const int n = a.C - wave * 64 * kRnEl;
+        return (float)(n < 0 ? 0 : n < 64 * kRnEl ? n : 64 * kRnEl);
+    };
+    TeamSums ts{lds, 0, 0.0f, 0.0f};
+    if (!in_wave(TEAM)) {
+        ts.per_wave = 1.0f / channels_of((int)threadIdx.x >> 6);
+        ts.in_lane = channels_of((int)threadIdx.x & 15);
+    }
     const long lo = (long)blockIdx.x * a.rows_blk;
     const long hi = lo + a.rows_blk < a.rows ? lo + a.rows_blk : a.rows;
     long row = lo + (in_wave(TEAM) ? (int)threadIdx.x / T : 0);
@@ -360,17 +363,17 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_k
     const f32x8 gq = load_param<MODE>(a.gq, 1.0f, k);
     const f32x8 bq = load_param<MODE>(a.bq, 0.0f, k);
     f32x8 phi = splat(1.0f), slope;
-    long have = -1;   // the gate row phi holds
+    long until = -1;   // the row from which phi is that of another gate row
     for (; row < hi; row += teams) {
         if (row + teams < hi) next.load(a, row + teams, k);
         f32x8 y = now.y.value(), h = now.x.value();
         if (OWN) {
             gate8(now.gate.value(), a.act, phi, slope);
         } else if (a.gate_rows) {
-            const long g = gate_row(row, a.gate_rows);
-            if (g != have) {
+            if (row >= until) {
+                const long g = gate_row(row, a.gate_rows);
                 gate8(load8<MODE>(static_cast<const YT*>(a.gate) + g * a.ldg, k), a.act, phi, slope);
-                have = g;
+                until = (g + 1) * a.gate_rows;
             }
         }
         float mean, rstd;
@@ -437,9 +440,9 @@ struct RnRow {
 // ahead and spilled registers 137, with a gate per row 177 against 253).
 template <typename YT, typename XT, bool OWN, int TEAM, int MODE>
 __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_kernel(RnBwd a) {
-    __shared__ double2 lds[in_wave(TEAM) ? 1 : 32];
+    __shared__ float2 lds[in_wave(TEAM) ? 1 : 32];
     __shared__ float fold[in_wave(TEAM) ? kRnThreads / 64 : 1][4][in_wave(TEAM) ? TEAM * kRnEl : 1];
-    TeamSums ts{lds, 0, 0.0};
+    TeamSums ts{lds, 0, 0.0f, 0.0f};
     const int T = team_size<TEAM>();
     const int t = in_wave(TEAM) ? (int)threadIdx.x % T : (int)threadIdx.x;
     const int teams = in_wave(TEAM) ? kRnThreads / T : 1;
@@ -493,8 +496,8 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
             const f32x8 hhat = (fma8(fma8(y, A, B), phi, now.x.value()) - now.ph) * now.rh;
             q0 += w;
             q1 = fma8(w, hhat, q1);
-            w = inside<MODE>(w * gq, k);
-            float m1 = sum8(w), m2 = sum8(w * hhat);
+            w = w * gq;
+            float m1 = own_sum<MODE>(w, k), m2 = own_sum<MODE>(w * hhat, k);
             team_sum2<TEAM>(m1, m2, ts);
             m1 = a.layer ? m1 * a.inv_c : 0.0f;
             m2 *= a.inv_c;
@@ -509,14 +512,13 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
             }
             store8<MODE>(static_cast<YT*>(a.dgate) + row * a.lddg, k, d * fma8(y, A, B) * slope);
         }
-        d = inside<MODE>(d, k);
         const f32x8 u = d * phi;
         const f32x8 keep = OWN ? u : d;
         p0 += keep;
         p1 = fma8(keep, y, p1);
         f32x8 w = u * A;
         if (a.post) {
-            float n1 = sum8(w), n2 = sum8(w * y);
+            float n1 = own_sum<MODE>(w, k), n2 = own_sum<MODE>(w * y, k);
             team_sum2<TEAM>(n1, n2, ts);
             n1 = a.layer ? n1 * a.inv_c : 0.0f;
             n2 *= a.inv_c;
@@ -801,7 +803,8 @@ static int32_t check_desc(const char* what, const pe_rnorm_desc* d) {
                d->x_dtype);
     PE_REQUIRE(d->norm == PE_RNORM_LAYER || d->norm == PE_RNORM_RMS, PE_E_UNSUPPORTED,
                "%s: unknown norm %d", what, d->norm);
-    PE_REQUIRE(d->eps > 0.0f && isfinite(d->eps), PE_E_INVALID, "%s: eps must be positive", what);
+    PE_REQUIRE(d->eps >= FLT_MIN && isfinite(d->eps), PE_E_INVALID,
+               "%s: eps must be positive and a normal number", what);
     PE_REQUIRE(d->gate_rows >= 0 && (d->gate_rows == 0 || d->rows % d->gate_rows == 0), PE_E_INVALID,
                "%s: %lld rows are not whole groups of %lld", what, (long long)d->rows,
                (long long)d->gate_rows);
@@ -938,7 +941,6 @@ extern "C" int32_t pe_rnorm_fwd(const pe_rnorm_desc* d, const void* y, const voi
     a.ldz = d->ldz;
     a.eps = d->eps;
     a.inv_c = 1.0f / (float)d->C;
-    a.inv_c64 = 1.0 / (double)d->C;
     a.C = d->C;
     a.post = d->post;
     a.pre = d->pre;
