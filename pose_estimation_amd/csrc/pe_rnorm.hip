@@ -118,17 +118,15 @@ struct Raw;
 template <int MODE>
 struct Raw<float, MODE> {
     f32x4 a, b;
-    __device__ __forceinline__ void load(const float* p, const Cols<MODE>& k, bool use = true) {
-        a = b = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (use) {
-            if (MODE == FEW) {
-                a.x = p[k.c];
-            } else {
-                a = *reinterpret_cast<const f32x4_any*>(p + k.c);
-                b = *reinterpret_cast<const f32x4_any*>(p + k.c + 4);
-            }
+    __device__ __forceinline__ void load(const float* p, const Cols<MODE>& k) {
+        if (MODE == FEW) {
+            a = b = f32x4{p[k.c], 0.0f, 0.0f, 0.0f};
+        } else {
+            a = *reinterpret_cast<const f32x4_any*>(p + k.c);
+            b = *reinterpret_cast<const f32x4_any*>(p + k.c + 4);
         }
     }
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(a), "+v"(b)); }
     __device__ __forceinline__ f32x8 value() const {
         return f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     }
@@ -137,16 +135,14 @@ struct Raw<float, MODE> {
 template <int MODE>
 struct Raw<uint16_t, MODE> {
     u32x4 v;
-    __device__ __forceinline__ void load(const uint16_t* p, const Cols<MODE>& k, bool use = true) {
-        v = u32x4{0, 0, 0, 0};
-        if (use) {
-            if (MODE == FEW) {
-                v.x = p[k.c];
-            } else {
-                v = *reinterpret_cast<const u32x4_any*>(p + k.c);
-            }
+    __device__ __forceinline__ void load(const uint16_t* p, const Cols<MODE>& k) {
+        if (MODE == FEW) {
+            v = u32x4{p[k.c], 0, 0, 0};
+        } else {
+            v = *reinterpret_cast<const u32x4_any*>(p + k.c);
         }
     }
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(v)); }
     __device__ __forceinline__ f32x8 value() const {
         f32x8 f;
 #pragma unroll
@@ -165,38 +161,47 @@ __device__ __forceinline__ f32x8 load8(const T* p, const Cols<MODE>& k) {
     return r.value();
 }
 
-template <int MODE>
+// ALL: also by threads whose channels are another's as well, which hold the same bits for them (and
+// have read them before, inside one wave, where the output may be the input).
+template <int MODE, bool ALL = false>
 __device__ __forceinline__ void store8(float* p, const Cols<MODE>& k, f32x8 f) {
-    if (MODE != FEW && k.on && k.first == 0) {
-        *reinterpret_cast<f32x4_any*>(p + k.c) = f32x4{f[0], f[1], f[2], f[3]};
-        *reinterpret_cast<f32x4_any*>(p + k.c + 4) = f32x4{f[4], f[5], f[6], f[7]};
-    } else if (MODE != WHOLE) {
+    if (MODE == FEW) {
+        if (ALL || k.on) p[k.c] = f[0];
+    } else if (ALL || (k.on && k.first == 0)) {
+        *reinterpret_cast<f32x4_any*>(p + k.c) = f.lo;
+        *reinterpret_cast<f32x4_any*>(p + k.c + 4) = f.hi;
+    } else if (MODE == TAIL) {
 #pragma unroll
         for (int j = 0; j < kRnEl; ++j)
             if (k.mine(j)) p[k.c + j] = f[j];
     }
 }
 
-template <int MODE>
+template <int MODE, bool ALL = false>
 __device__ __forceinline__ void store8(uint16_t* p, const Cols<MODE>& k, f32x8 f) {
     u32x4 v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = pack_bf16x2_bits(f[2 * j], f[2 * j + 1]);
-    if (MODE != FEW && k.on && k.first == 0) {
+    if (MODE == FEW) {
+        if (ALL || k.on) p[k.c] = (uint16_t)v[0];
+    } else if (ALL || (k.on && k.first == 0)) {
         *reinterpret_cast<u32x4_any*>(p + k.c) = v;
-    } else if (MODE != WHOLE) {
+    } else if (MODE == TAIL) {
 #pragma unroll
         for (int j = 0; j < kRnEl; ++j)
             if (k.mine(j)) p[k.c + j] = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
     }
 }
 
+// The last thread's neighbour may be in another wave of a workgroup.
+constexpr bool store_all(int team, int mode) { return in_wave(team) || mode == WHOLE; }
+
 template <int MODE>
 __device__ __forceinline__ f32x8 load_param(const float* p, float absent, const Cols<MODE>& k) {
     return p ? load8<MODE>(p, k) : splat(absent);
 }
 
-// A thread's share of a sum over the row, and of a sum of squares.
+// A thread's share of a sum over the row, and of a sum of products: of its own channels.
 template <int MODE>
 __device__ __forceinline__ f32x8 own(f32x8 v, const Cols<MODE>& k) {
     if (MODE == WHOLE) return v;
@@ -206,16 +211,15 @@ __device__ __forceinline__ f32x8 own(f32x8 v, const Cols<MODE>& k) {
 }
 
 template <int MODE>
-__device__ __forceinline__ float own_sum(f32x8 v, const Cols<MODE>& k) {
-    v = own<MODE>(v, k);
-    const float s = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+__device__ __forceinline__ float sum8(f32x8 own_v, const Cols<MODE>& k) {
+    const f32x4 q = own_v.lo + own_v.hi;
+    const float s = (q[0] + q[1]) + (q[2] + q[3]);
     return MODE != WHOLE || k.on ? s : 0.0f;
 }
 
 template <int MODE>
-__device__ __forceinline__ float own_squares(f32x8 v, const Cols<MODE>& k) {
-    v = own<MODE>(v, k);
-    const f32x4 q = __builtin_elementwise_fma(v.hi, v.hi, v.lo * v.lo);
+__device__ __forceinline__ float dot8(f32x8 own_v, f32x8 w, const Cols<MODE>& k) {
+    const f32x4 q = __builtin_elementwise_fma(own_v.hi, w.hi, own_v.lo * w.lo);
     const float s = (q[0] + q[1]) + (q[2] + q[3]);
     return MODE != WHOLE || k.on ? s : 0.0f;
 }
@@ -226,10 +230,13 @@ __device__ __forceinline__ float own_squares(f32x8 v, const Cols<MODE>& k) {
 // one barrier a sum is enough.
 struct TeamSums {
     float2* buf;    // LDS [2][16], workgroup teams only
-    int turn;
+    int waves, turn;
     // 1 / this wave's channels, and the channels of the wave of the lane's index; forward only
     float per_wave, in_lane;
 };
+
+// Of a workgroup that works on one row.
+__host__ __device__ constexpr int waves_of(int C) { return (C + 64 * kRnEl - 1) / (64 * kRnEl); }
 
 __device__ __forceinline__ float2 each_wave(float2 v, TeamSums& ts) {
     float2* buf = ts.buf + 16 * ts.turn;
@@ -238,7 +245,7 @@ __device__ __forceinline__ float2 each_wave(float2 v, TeamSums& ts) {
     __syncthreads();
     const int w = (int)threadIdx.x & 15;
     v = buf[w];
-    return w < (int)blockDim.x >> 6 ? v : float2{0.0f, 0.0f};
+    return w < ts.waves ? v : float2{0.0f, 0.0f};
 }
 
 template <int TEAM>
@@ -264,10 +271,11 @@ __device__ __forceinline__ void normalise(f32x8& v, const Cols<MODE>& k, float i
     mean = 0.0f;
     f32x8 c = v;
     if (layer) {
-        mean = lanes_sum<W>(own_sum<MODE>(v, k)) * (in_wave(TEAM) ? inv_c : ts.per_wave);
+        mean = lanes_sum<W>(sum8(own<MODE>(v, k), k)) * (in_wave(TEAM) ? inv_c : ts.per_wave);
         c = v - mean;
     }
-    float var = lanes_sum<W>(own_squares<MODE>(c, k)), shift = 0.0f;
+    const f32x8 own_c = own<MODE>(c, k);
+    float var = lanes_sum<W>(dot8(own_c, own_c, k)), shift = 0.0f;
     if (!in_wave(TEAM)) {
         const float own_mean = mean;
         const float2 w = each_wave(float2{mean, var}, ts);
@@ -323,17 +331,47 @@ __device__ __forceinline__ long gate_row(long row, long per) {
     return row / per;
 }
 
+// ---- rows ---------------------------------------------------------------------------------
+// Every load of a row is made, and its stores too where they can be: the compiler waits for loads
+// by the number of accesses that are sure to come after them, so a branch around any of these
+// would make each row wait for the next one's loads.  What is absent is a row of zeros, and past
+// its last row a team reads that one again.
+__device__ float rn_zeros[kRnMaxC];
+
+template <typename T>
+struct Rows {
+    const T* p;
+    long ld;
+    __device__ __forceinline__ Rows(const void* at, long stride) {
+        p = at ? static_cast<const T*>(at) : reinterpret_cast<const T*>(rn_zeros);
+        ld = at ? stride : 0;
+    }
+    __device__ __forceinline__ const T* operator[](long row) const { return p + row * ld; }
+};
+
+// step(row, this row's data, the next one's) for the rows of a team from `row` on to hi; two sets
+// of registers in turn.
+template <typename ROW, typename LOAD, typename STEP>
+__device__ __forceinline__ void for_rows(long row, long hi, int teams, LOAD load, STEP step) {
+    ROW one, two;
+    if (row < hi) load(one, row);
+    while (row < hi) {
+        load(two, row + teams < hi ? row + teams : hi - 1);
+        step(row, one);
+        row += teams;
+        if (row >= hi) break;
+        load(one, row + teams < hi ? row + teams : hi - 1);
+        step(row, two);
+        row += teams;
+    }
+}
+
 // ---- forward ------------------------------------------------------------------------------
 // OWN: a gate row for each row.  The next row is loaded while this one is worked on.
 template <typename YT, typename XT, bool OWN, int MODE>
 struct FwdRow {
     Raw<YT, MODE> y, gate;
     Raw<XT, MODE> x;
-    __device__ __forceinline__ void load(const RnFwd& a, long row, const Cols<MODE>& k) {
-        y.load(static_cast<const YT*>(a.y) + row * a.ldy, k);
-        x.load(static_cast<const XT*>(a.x) + row * a.ldx, k, a.x);
-        if (OWN) gate.load(static_cast<const YT*>(a.gate) + row * a.ldg, k);
-    }
 };
 
 template <typename YT, typename XT, bool OWN, int TEAM, int MODE>
@@ -347,7 +385,7 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_k
         const int n = a.C - wave * 64 * kRnEl;
         return (float)(n < 0 ? 0 : n < 64 * kRnEl ? n : 64 * kRnEl);
     };
-    TeamSums ts{lds, 0, 0.0f, 0.0f};
+    TeamSums ts{lds, waves_of(a.C), 0, 0.0f, 0.0f};
     if (!in_wave(TEAM)) {
         ts.per_wave = 1.0f / channels_of((int)threadIdx.x >> 6);
         ts.in_lane = channels_of((int)threadIdx.x & 15);
@@ -355,8 +393,8 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_k
     const long lo = (long)blockIdx.x * a.rows_blk;
     const long hi = lo + a.rows_blk < a.rows ? lo + a.rows_blk : a.rows;
     long row = lo + (in_wave(TEAM) ? (int)threadIdx.x / T : 0);
-    FwdRow<YT, XT, OWN, MODE> now, next;
-    if (row < hi) now.load(a, row, k);
+    const Rows<YT> ys(a.y, a.ldy), gates(a.gate, a.ldg);
+    const Rows<XT> xs(a.x, a.ldx);
     const f32x8 s = load_param<MODE>(a.s, 1.0f, k);
     const f32x8 A = load_param<MODE>(a.gp, 1.0f, k) * s;
     const f32x8 B = load_param<MODE>(a.bp, 0.0f, k) * s;
@@ -364,15 +402,20 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_k
     const f32x8 bq = load_param<MODE>(a.bq, 0.0f, k);
     f32x8 phi = splat(1.0f), slope;
     long until = -1;   // the row from which phi is that of another gate row
-    for (; row < hi; row += teams) {
-        if (row + teams < hi) next.load(a, row + teams, k);
+    typedef FwdRow<YT, XT, OWN, MODE> Row;
+    auto load = [&](Row& r, long at) {
+        r.y.load(ys[at], k);
+        r.x.load(xs[at], k);
+        if (OWN) r.gate.load(gates[at], k);
+    };
+    for_rows<Row>(row, hi, teams, load, [&](long row, const Row& now) {
         f32x8 y = now.y.value(), h = now.x.value();
         if (OWN) {
             gate8(now.gate.value(), a.act, phi, slope);
         } else if (a.gate_rows) {
             if (row >= until) {
                 const long g = gate_row(row, a.gate_rows);
-                gate8(load8<MODE>(static_cast<const YT*>(a.gate) + g * a.ldg, k), a.act, phi, slope);
+                gate8(load8<MODE>(gates[g], k), a.act, phi, slope);
                 until = (g + 1) * a.gate_rows;
             }
         }
@@ -385,17 +428,16 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_k
             }
         }
         h = fma8(fma8(y, A, B), phi, h);
-        store8<MODE>(static_cast<XT*>(a.h) + row * a.ldh, k, h);
+        store8<MODE, store_all(TEAM, MODE)>(static_cast<XT*>(a.h) + row * a.ldh, k, h);
         if (a.pre) {
             normalise<TEAM, MODE>(h, k, a.inv_c, a.eps, a.layer, mean, rstd, ts);
             if (a.stats && t == 0) {
                 if (a.layer) a.stats[2 * a.rows + row] = mean;
                 a.stats[3 * a.rows + row] = rstd;
             }
-            store8<MODE>(static_cast<YT*>(a.z) + row * a.ldz, k, fma8(h, gq, bq));
+            store8<MODE, store_all(TEAM, MODE)>(static_cast<YT*>(a.z) + row * a.ldz, k, fma8(h, gq, bq));
         }
-        now = next;
-    }
+    });
 }
 
 // ---- backward -----------------------------------------------------------------------------
@@ -410,28 +452,10 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_k
 // crosses a gate row: phi is a constant of the item, which leaves its sums of D with phi (for the
 // parameters) and without (for the gate).  A gate row for each row has its gradient in the loop.
 template <typename YT, typename XT, bool OWN, int MODE>
-struct RnRow {
+struct BwdRow {
     Raw<YT, MODE> y, dz, gate;
     Raw<XT, MODE> x, dh;
     float py, ry, ph, rh;   // mean and rstd of y and of h
-    // What is absent reads as 0 (x, dh) or is not looked at (the rest).
-    __device__ __forceinline__ void load(const RnBwd& a, long row, const Cols<MODE>& k) {
-        y.load(static_cast<const YT*>(a.y) + row * a.ldy, k);
-        x.load(static_cast<const XT*>(a.x) + row * a.ldx, k, a.x && a.pre);
-        dh.load(static_cast<const XT*>(a.dh) + row * a.lddh, k, a.dh);
-        py = ph = 0.0f;
-        ry = rh = 1.0f;
-        if (a.pre) {
-            dz.load(static_cast<const YT*>(a.dz) + row * a.lddz, k);
-            rh = a.stats[3 * a.rows + row];
-            if (a.layer) ph = a.stats[2 * a.rows + row];
-        }
-        if (a.post) {
-            ry = a.stats[a.rows + row];
-            if (a.layer) py = a.stats[row];
-        }
-        if (OWN) gate.load(static_cast<const YT*>(a.gate) + row * a.ldg, k);
-    }
 };
 
 // OWN: a gate row for each row.  The next row is loaded while this one is worked on.  Workgroups
@@ -439,15 +463,16 @@ struct RnRow {
 // no row ahead (4000 x 8192 bf16: 117 us; with the parameters in registers 127, with the row
 // ahead and spilled registers 137, with a gate per row 177 against 253).
 template <typename YT, typename XT, bool OWN, int TEAM, int MODE>
-__global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_kernel(RnBwd a) {
+__global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM,
+                             TEAM == 512 && sizeof(XT) == 2 ? 3 : 1) void rnorm_bwd_kernel(RnBwd a) {
     __shared__ float2 lds[in_wave(TEAM) ? 1 : 32];
     __shared__ float fold[in_wave(TEAM) ? kRnThreads / 64 : 1][4][in_wave(TEAM) ? TEAM * kRnEl : 1];
-    TeamSums ts{lds, 0, 0.0f, 0.0f};
+    TeamSums ts{lds, waves_of(a.C), 0, 0.0f, 0.0f};
     const int T = team_size<TEAM>();
     const int t = in_wave(TEAM) ? (int)threadIdx.x % T : (int)threadIdx.x;
     const int teams = in_wave(TEAM) ? kRnThreads / T : 1;
     const Cols<MODE> k(t, a.C);
-    constexpr bool WIDE = TEAM == 1024;
+    constexpr bool WIDE = TEAM == 1024, ALL = !WIDE && store_all(TEAM, MODE);
     __shared__ f32x4 held[WIDE ? 6 : 1][WIDE ? 1024 : 1];   // each thread's own, no barrier
     const f32x8 s = load_param<MODE>(a.s, 1.0f, k);
     f32x8 A = load_param<MODE>(a.gp, 1.0f, k) * s;
@@ -463,72 +488,102 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
         v.hi = held[2 * i + 1][threadIdx.x];
         return v;
     };
+    const long g = (long)blockIdx.x / a.nseg;
+    const long lo = g * a.group + ((long)blockIdx.x - g * a.nseg) * a.rows_blk;
+    const long end = (g + 1) * a.group;
+    const long hi = lo + a.rows_blk < end ? lo + a.rows_blk : end;
+    const bool shared = !OWN && a.gate_rows;
+    const YT* item_gate = static_cast<const YT*>(a.gate) + g * a.ldg;   // of a shared gate
+    f32x8 phi, slope;
+    if (shared) {
+        gate8(load8<MODE>(item_gate, k), a.act, phi, slope);
+        A *= phi;
+        B *= phi;
+    }
     if (WIDE) {
         hold(0, A);
         hold(1, B);
         hold(2, gq);
     }
-    f32x8 phi = splat(1.0f), slope = splat(1.0f);
-    const long g = (long)blockIdx.x / a.nseg;
-    const long lo = g * a.group + ((long)blockIdx.x - g * a.nseg) * a.rows_blk;
-    const long end = (g + 1) * a.group;
-    const long hi = lo + a.rows_blk < end ? lo + a.rows_blk : end;
-    if (!OWN && a.gate_rows)
-        gate8(load8<MODE>(static_cast<const YT*>(a.gate) + g * a.ldg, k), a.act, phi, slope);
     f32x8 q1 = splat(0.0f), q0 = q1, p1 = q1, p0 = q1;
     long row = lo + (in_wave(TEAM) ? (int)threadIdx.x / T : 0);
-    RnRow<YT, XT, OWN, MODE> now, next;
-    constexpr bool AHEAD = !WIDE;
-    if (AHEAD && row < hi) now.load(a, row, k);
-    for (; row < hi; row += teams) {
-        if (!AHEAD) now.load(a, row, k);
-        if (AHEAD && row + teams < hi) next.load(a, row + teams, k);
+    const Rows<YT> ys(a.y, a.ldy), dzs(a.pre ? a.dz : nullptr, a.lddz), gates(a.gate, a.ldg);
+    const Rows<XT> xs(a.pre ? a.x : nullptr, a.ldx), dhs(a.dh, a.lddh);
+    // the planes of the statistics, as rows of one element
+    const Rows<float> pys(a.post && a.layer ? a.stats : nullptr, 1), rys(a.post ? a.stats + a.rows : nullptr, 1);
+    const Rows<float> phs(a.pre && a.layer ? a.stats + 2 * a.rows : nullptr, 1);
+    const Rows<float> rhs(a.pre ? a.stats + 3 * a.rows : nullptr, 1);
+    typedef BwdRow<YT, XT, OWN, MODE> Row;
+    auto load = [&](Row& r, long at) {
+        r.y.load(ys[at], k);
+        r.x.load(xs[at], k);
+        r.dh.load(dhs[at], k);
+        r.dz.load(dzs[at], k);
+        if (OWN) r.gate.load(gates[at], k);
+        r.py = *pys[at];
+        r.ry = *rys[at];
+        r.ph = *phs[at];
+        r.rh = *rhs[at];
+    };
+    auto step = [&](long row, const Row& now) {
         f32x8 y = now.y.value(), d = now.dh.value();
         if (OWN) gate8(now.gate.value(), a.act, phi, slope);
-        if (a.post) y = (y - now.py) * now.ry;
+        if (a.post) y = fma8(y, splat(now.ry), splat(-now.py * now.ry));
         if (a.pre) {
             if (WIDE) {
                 A = held8(0);
                 B = held8(1);
                 gq = held8(2);
             }
-            f32x8 w = now.dz.value();
-            const f32x8 hhat = (fma8(fma8(y, A, B), phi, now.x.value()) - now.ph) * now.rh;
+            f32x8 w = now.dz.value(), h = fma8(y, A, B);
+            h = OWN ? fma8(h, phi, now.x.value()) : now.x.value() + h;
+            const f32x8 hhat = fma8(h, splat(now.rh), splat(-now.ph * now.rh));
             q0 += w;
             q1 = fma8(w, hhat, q1);
             w = w * gq;
-            float m1 = own_sum<MODE>(w, k), m2 = own_sum<MODE>(w * hhat, k);
+            const f32x8 own_w = own<MODE>(w, k);
+            float m1 = sum8(own_w, k), m2 = dot8(own_w, hhat, k);
             team_sum2<TEAM>(m1, m2, ts);
             m1 = a.layer ? m1 * a.inv_c : 0.0f;
             m2 *= a.inv_c;
             d = fma8(fma8(hhat, splat(-m2), w - m1), splat(now.rh), d);
         }
-        if (a.dx) store8<MODE>(static_cast<XT*>(a.dx) + row * a.lddx, k, d);
+        if (a.dx) store8<MODE, ALL>(static_cast<XT*>(a.dx) + row * a.lddx, k, d);
         if (WIDE) A = held8(0);
         if (OWN) {
-            if (WIDE) {   // again, rather than kept over the sum
-                B = held8(1);
-                gate8(now.gate.value(), a.act, phi, slope);
+            if (WIDE) B = held8(1);
+            if (!in_wave(TEAM)) {   // again, rather than kept over the sum
+                Raw<YT, MODE> gate = now.gate;
+                gate.forget();
+                gate8(gate.value(), a.act, phi, slope);
             }
-            store8<MODE>(static_cast<YT*>(a.dgate) + row * a.lddg, k, d * fma8(y, A, B) * slope);
+            store8<MODE, ALL>(static_cast<YT*>(a.dgate) + row * a.lddg, k, d * fma8(y, A, B) * slope);
+            d *= phi;
         }
-        const f32x8 u = d * phi;
-        const f32x8 keep = OWN ? u : d;
-        p0 += keep;
-        p1 = fma8(keep, y, p1);
-        f32x8 w = u * A;
+        p0 += d;
+        p1 = fma8(d, y, p1);
+        f32x8 w = d * A;
         if (a.post) {
-            float n1 = own_sum<MODE>(w, k), n2 = own_sum<MODE>(w * y, k);
+            const f32x8 own_w = own<MODE>(w, k);
+            float n1 = sum8(own_w, k), n2 = dot8(own_w, y, k);
             team_sum2<TEAM>(n1, n2, ts);
-            n1 = a.layer ? n1 * a.inv_c : 0.0f;
-            n2 *= a.inv_c;
-            w = fma8(y, splat(-n2), w - n1) * now.ry;
+            n1 = a.layer ? n1 * a.inv_c * now.ry : 0.0f;
+            n2 *= a.inv_c * now.ry;
+            w = fma8(y, splat(-n2), fma8(w, splat(now.ry), splat(-n1)));
         }
-        store8<MODE>(static_cast<YT*>(a.dy) + row * a.lddy, k, w);
-        if (AHEAD) now = next;
+        store8<MODE, ALL>(static_cast<YT*>(a.dy) + row * a.lddy, k, w);
+    };
+    if (WIDE) {
+        for (; row < hi; row += teams) {
+            Row now;
+            load(now, row);
+            step(row, now);
+        }
+    } else {
+        for_rows<Row>(row, hi, teams, load, step);
     }
     if (!a.need) return;
-    const bool shared = !OWN && a.gate_rows, direct = a.part == nullptr;
+    const bool direct = a.part == nullptr;
     float* out = direct ? nullptr : a.part + (long)blockIdx.x * slots_of(a.gate_rows) * a.pitch;
     if (in_wave(TEAM)) {
         // rows side by side in the wave, then the waves in order
@@ -549,7 +604,7 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
         __syncthreads();
         for (int c = threadIdx.x; c < a.C; c += kRnThreads) {
             float f = 1.0f, unused;
-            if (shared) f = gate_value(as_float(static_cast<const YT*>(a.gate)[g * a.ldg + c]), a.act, unused);
+            if (shared) f = gate_value(as_float(item_gate[c]), a.act, unused);
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -584,7 +639,8 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_bwd_k
             store8<MODE>(a.ds, k, v);
         }
     } else {
-        const f32x8 f = shared ? phi : splat(1.0f);
+        f32x8 f = splat(1.0f);
+        if (shared) gate8(load8<MODE>(item_gate, k), a.act, f, slope);
         if (a.need & kQ1) store8<MODE>(out, k, q1);
         if (a.need & kQ0) store8<MODE>(out + a.pitch, k, q0);
         if (a.need & kP1) store8<MODE>(out + 2l * a.pitch, k, p1 * f);
@@ -749,7 +805,7 @@ static int team_of(int C) {
 }
 
 static unsigned block_of(int C) {   // threads of a workgroup
-    return in_wave(team_of(C)) ? kRnThreads : (unsigned)(((C + kRnEl - 1) / kRnEl + 63) / 64 * 64);
+    return in_wave(team_of(C)) ? kRnThreads : 64u * waves_of(C);
 }
 
 static long rows_at_once(int C) { return in_wave(team_of(C)) ? kRnThreads / team_of(C) : 1; }
