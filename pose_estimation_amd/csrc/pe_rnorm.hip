@@ -827,7 +827,8 @@ static BwdGeom bwd_geom(const pe_rnorm_desc& d) {
     const long at_once = rows_at_once(d.C);
     long want = kRnItems * 256 / (long)block_of(d.C);
     if (want > d.rows / 8) want = d.rows / 8;
-    if (want < kRnItems) want = kRnItems;
+    const long least = waves_of(d.C) > 6 ? kRnItems / 2 : kRnItems;
+    if (want < least) want = least;
     want = (want + g.groups - 1) / g.groups;
     long rows = (g.group + want - 1) / want;
     rows = (rows + at_once - 1) / at_once * at_once;
