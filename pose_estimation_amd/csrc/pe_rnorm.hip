@@ -1011,7 +1011,8 @@ extern "C" int32_t pe_rnorm_fwd(const pe_rnorm_desc* d, const void* y, const voi
     const long at_once = rows_at_once(d->C);
     long rows = (d->rows + 4095) / 4096;
     if (!in_wave(team_of(d->C))) {
-        const long round = (1l << 18) / block_of(d->C);
+        const long per_cu = (d->x_dtype == PE_DTYPE_F32 ? 16 : 20) / waves_of(d->C);   // by registers
+        const long round = 256 * (per_cu > 1 ? per_cu : 1);
         const long yb = d->y_dtype == PE_DTYPE_F32 ? 4 : 2, xb = d->x_dtype == PE_DTYPE_F32 ? 4 : 2;
         const long params = 4 * ((post_gamma != nullptr) + (post_beta != nullptr) + (scale != nullptr) +
                                  (pre_gamma != nullptr) + (pre_beta != nullptr));
