@@ -275,21 +275,20 @@ __device__ __forceinline__ void normalise(f32x8& v, const Cols<MODE>& k, float i
         c = v - mean;
     }
     const f32x8 own_c = own<MODE>(c, k);
-    float var = lanes_sum<W>(dot8(own_c, own_c, k)), shift = 0.0f;
+    float var = lanes_sum<W>(dot8(own_c, own_c, k));
     if (!in_wave(TEAM)) {
-        const float own_mean = mean;
         const float2 w = each_wave(float2{mean, var}, ts);
         if (layer) {
             mean = lanes_sum<16>(w.x * ts.in_lane) * inv_c;
             const float d = w.x - mean;
             var = lanes_sum<16>(__builtin_fmaf(d * ts.in_lane, d, w.y));
-            shift = own_mean - mean;
+            c = v - mean;
         } else {
             var = lanes_sum<16>(w.y);
         }
     }
     rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(var, inv_c, eps));   // good to 2^-23; eps is normal
-    v = in_wave(TEAM) ? c * rstd : fma8(c, splat(rstd), splat(shift * rstd));
+    v = c * rstd;
 }
 
 // ---- gate ---------------------------------------------------------------------------------
@@ -528,7 +527,7 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM,
     auto step = [&](long row, const Row& now) {
         f32x8 y = now.y.value(), d = now.dh.value();
         if (OWN) gate8(now.gate.value(), a.act, phi, slope);
-        if (a.post) y = fma8(y, splat(now.ry), splat(-now.py * now.ry));
+        if (a.post) y = (y - now.py) * now.ry;
         if (a.pre) {
             if (WIDE) {
                 A = held8(0);
@@ -537,7 +536,7 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM,
             }
             f32x8 w = now.dz.value(), h = fma8(y, A, B);
             h = OWN ? fma8(h, phi, now.x.value()) : now.x.value() + h;
-            const f32x8 hhat = fma8(h, splat(now.rh), splat(-now.ph * now.rh));
+            const f32x8 hhat = (h - now.ph) * now.rh;
             q0 += w;
             q1 = fma8(w, hhat, q1);
             w = w * gq;

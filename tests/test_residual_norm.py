@@ -550,6 +550,47 @@ def test_in_place_and_repeated_calls_give_the_same_bits(C, post):
 
 
 @gpu
+@pytest.mark.parametrize("C", [3, 44, 513, 516, 1030, 4100])
+@pytest.mark.parametrize("post", [None, "gb"])
+@pytest.mark.parametrize("pre", [None, "gb"])
+def test_in_place_where_threads_share_channels(C, post, pre, monkeypatch):
+    """Both directions at widths whose last channels belong to two threads, in two waves where a
+    row takes more than one."""
+    t = make(300, C, "bf16", post, pre, gate="row")
+    want = call(t, "layer", "silu")
+    kw = dict(norm="layer", post=t["post"], pre=t["pre"], scale=t["scale"], gate=t["gate"],
+              gate_act="silu")
+    stats = nn.residual_norm(t["y"], t["x"], want_stats=True, **kw)[2]
+    dh, dz = t["dh"].clone(), None if pre is None else t["dz"].clone()
+    dy = torch.empty_like(t["y"]) if dz is None else dz
+    fresh = iter([dy, dh, torch.empty_like(t["gate"])])   # dy, dx, dgate
+    with monkeypatch.context() as m:
+        m.setattr(nn, "_dense_like", lambda like: next(fresh))
+        got = nn.residual_norm_bwd(dh, dz, t["y"], t["x"], stats, **kw)
+    for k, v in got.items():
+        assert v is want[k] is None or torch.equal(v, want[k]), k
+    y, x = t["y"].clone(), t["x"].clone()
+    nn.residual_norm(y, x, out=(x, y if pre else None), **kw)
+    assert torch.equal(x, want["h"]) and (pre is None or torch.equal(y, want["z"]))
+
+
+@gpu
+@pytest.mark.parametrize("C", [24, 333, 520, 1048, 4100])
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+def test_rows_far_from_zero_and_lopsided_rows(C, norm):
+    """A mean far above the spread, and rows whose first or last few channels are far from the
+    rest, so that the parts of a row that are summed apart have means of their own."""
+    t = make(12, C, "f32")
+    t["y"][:4] += 1000.0
+    t["y"][4:6, :8] += 500.0
+    t["y"][6:8, -8:] += 500.0
+    t["y"][8, -1] = 4000.0
+    t["x"][9] -= 1000.0
+    t["x"][10, -8:] += 300.0
+    check(t, norm)
+
+
+@gpu
 @pytest.mark.parametrize("C", [56, 1048])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_non_finite_values_stay_in_their_row(C, bad):
