@@ -28,12 +28,14 @@ namespace pe {
 constexpr int kRnMaxC = 8192;
 constexpr int kRnEl = 8;          // channels a thread holds
 constexpr int kRnThreads = 256;   // of a workgroup whose rows are shorter than a wave's reach
-// Items of backward (workgroups, each with a set of partial sums), about.  Two a CU: at 196608 x
-// 256 bf16 the launch takes 141, 129, 133, 145, 138 us with 256, 512, 768, 1024, 2048 of them, at
-// 3456 x 2048 29, 26, 28, 30, 35 us, and the fold behind it grows with their number.  More where a
-// row takes a workgroup of less than 256 threads, for as many threads in all (16000 x 1024: both
-// launches 55 us, with 512 items 68), as long as an item has eight rows (2000 x 1024: 23 us, 26).
-constexpr int kRnItems = 512;
+// Items of backward (workgroups, each with a set of partial sums), about: as many for each compute
+// unit, all of them there at once, few enough for the fold behind them.  Rows inside a wave: two
+// (both launches at 60000 x 333 bf16 66 us, with 1.5, 3, 4 a unit 75, 67, 70; at 196608 x 256 135,
+// 135, 139, 136).  A workgroup of 3 to 6 waves: two (10000 x 1400 45 us; 2.7, 4, 5.3 of them 49, 50, 57),
+// of more: one, which is all that its registers leave room for (3000 x 4096 38 us, with two 46), of 2:
+// four (60000 x 520 105 us, with three 119), or two where an item would not have eight rows
+// (2000 x 1024: 22 us, with four 26).
+constexpr long kRnUnits = 256;
 // The sums an item leaves, as bits of what anything needs: of dz*hhat, dz, D*phi*yhat and D*phi,
 // and with a gate shared by several rows also of D*yhat and D.
 enum { kQ1 = 1, kQ0 = 2, kP1 = 4, kP0 = 8, kG1 = 16, kG0 = 32 };
@@ -817,17 +819,16 @@ struct BwdGeom {
 
 static int pitch_of(int C) { return (C + 3) & ~3; }   // of a row of sums: 16-byte steps
 
-// About kRnItems items, none across a gate row, each a multiple of the rows its teams take at once.
+// None across a gate row, each a multiple of the rows its teams take at once.
 static BwdGeom bwd_geom(const pe_rnorm_desc& d) {
     BwdGeom g;
     const bool grouped = d.gate_rows > 1;
     g.group = grouped ? d.gate_rows : d.rows;
     g.groups = grouped ? d.rows / d.gate_rows : 1;
     const long at_once = rows_at_once(d.C);
-    long want = kRnItems * 256 / (long)block_of(d.C);
-    if (want > d.rows / 8) want = d.rows / 8;
-    const long least = waves_of(d.C) > 6 ? kRnItems / 2 : kRnItems;
-    if (want < least) want = least;
+    const int waves = waves_of(d.C);   // 1: rows inside a wave
+    long want = waves > 6 ? kRnUnits : 2 * kRnUnits;
+    if (waves == 2 && d.rows / 8 > want) want = d.rows / 8 < 4 * kRnUnits ? d.rows / 8 : 4 * kRnUnits;
     want = (want + g.groups - 1) / g.groups;
     long rows = (g.group + want - 1) / want;
     rows = (rows + at_once - 1) / at_once * at_once;
