@@ -1004,12 +1004,14 @@ extern "C" int32_t pe_rnorm_fwd(const pe_rnorm_desc* d, const void* y, const voi
     a.layer = d->norm == PE_RNORM_LAYER;
     a.act = d->gate_act;
     // Workgroups of equal shares, each of which loads the parameters once.  Rows inside a wave:
-    // 4096 of them (60000 x 333 bf16: 47 us, with 8192 51, with 2048 46; 196608 x 256 with a gate
-    // 83, 83, 83).  A row to a workgroup: whole rounds of what the chip holds at once, four (8192 x
-    // 4096 with a float32 residual, rms: 90 us, with two 94), or two or one where the parameters
-    // would be over half of the bytes (8000 x 4000 bf16, layer: two 62 us, four 66).
+    // 4096 of them (196608 x 256 bf16 76 us, with 1024 82; 70000 x 512 46, 48), or 1024 where the width
+    // is no multiple of eight (60000 x 333: 33 us, with 4096 38; 20000 x 333 12, 15).  A row to a
+    // workgroup: whole rounds of what the chip holds at once, four (8192 x 4096 with a float32
+    // residual, rms: 90 us, with two 94), or two or one where the parameters would be over half of
+    // the bytes.
     const long at_once = rows_at_once(d->C);
-    long rows = (d->rows + 4095) / 4096;
+    const long shares = d->C % kRnEl == 0 ? 4096 : 1024;
+    long rows = (d->rows + shares - 1) / shares;
     if (!in_wave(team_of(d->C))) {
         const long per_cu = (d->x_dtype == PE_DTYPE_F32 ? 16 : 20) / waves_of(d->C);   // by registers
         const long round = 256 * (per_cu > 1 ? per_cu : 1);
