@@ -721,7 +721,7 @@ int32_t pe_bn_bwd_bf16(const void* da, const void* a, int32_t relu, const void* 
  *   h = x + scale * phi(gate) * a                 x may be NULL (0)
  *   z = N(h)*pre_gamma + pre_beta                 only with pre
  *   N(v) = (v - mean)*rstd (PE_RNORM_LAYER) or v*rstd (PE_RNORM_RMS), over the row,
- *   rstd = 1/sqrt(mean((v - mean)^2) + eps) (mean 0 for RMS);  phi = identity, sigmoid or silu
+ *   rstd = 1/sqrt(mean((v - mean)^2) + eps) (mean 0 for RMS; eps at least 2^-126);  phi = identity, sigmoid or silu
  * y, gate, z and their gradients have y_dtype; x, h and theirs x_dtype: (bf16, bf16),
  * (bf16, f32) or (f32, f32).  z is the norm of h BEFORE h is rounded.  gammas, betas and scale are
  * float32 [C] or NULL (1, 0, 1).  gate holds one row for every gate_rows rows of y (1: a row of

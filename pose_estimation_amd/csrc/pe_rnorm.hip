@@ -8,13 +8,15 @@
 // it from its load to its store, so statistics, both norms and the gate cost no further pass.
 // Eight channels a thread (one 16-byte load of bf16): a team is the next power of two of C/8
 // threads inside one wave (1 to 64, several rows a wave side by side), or, past 512 channels, a
-// workgroup of its own.  Means and variances come from the registers, in two steps or from float64
-// sums (no difference of large float32 sums); all other arithmetic is float32, each output is
-// rounded once.  Wider shares of a row per thread would not leave a wave the registers to have
-// the next row under way, narrower ones add lanes to every sum.
-// Measured: forward 8192 x 4096 bf16 with a float32 residual and a gate per row 92 us (5.1 TB/s),
-// 196608 x 256 bf16 82 us (4.9 TB/s) and backward there 131 us (4.6 TB/s; a copy reaches 4.7),
-// one row of 4096 3.4 us.
+// workgroup of its own.  Means and variances come from the registers in two steps, so no large sums
+// cancel; all arithmetic is float32, each output is rounded once.  Wider shares of a row per thread
+// would not leave a wave the registers to have the next row under way, narrower ones add lanes to
+// every sum.  Where a last wave has little to do (just past 512, 1024, 2048, 4096 channels) the
+// vector instructions bound it instead, about 190 for eight channels forward, 350 backward.
+// Measured: forward 8192 x 4096 bf16 with a float32 residual and a gate per row 88 us (5.3 TB/s),
+// 196608 x 256 bf16 with a gate per image 74 us (5.5 TB/s) and backward there 128 us (4.7 TB/s, as a
+// copy), 8000 x 4096 bf16 46 us (5.7 TB/s) and backward with its fold 88 us (4.5 TB/s), one row of
+// 4096 3.2 us.
 #include <float.h>
 #include <math.h>
 
@@ -335,8 +337,9 @@ __device__ __forceinline__ long gate_row(long row, long per) {
 // ---- rows ---------------------------------------------------------------------------------
 // Every load of a row is made, and its stores too where they can be: the compiler waits for loads
 // by the number of accesses that are sure to come after them, so a branch around any of these
-// would make each row wait for the next one's loads.  What is absent is a row of zeros, and past
-// its last row a team reads that one again.
+// would make each row wait for the next one's loads (60000 x 333 bf16, backward: 66 us, with
+// branches 85).  What is absent is a row of zeros, and past its last row a team reads that one again
+// (zeros instead: 5 % fewer bytes at 8192 x 4096, but 8000 x 4096 backward 97 us, not 88).
 __device__ float rn_zeros[kRnMaxC];
 
 template <typename T>
@@ -350,8 +353,8 @@ struct Rows {
     __device__ __forceinline__ const T* operator[](long row) const { return p + row * ld; }
 };
 
-// step(row, this row's data, the next one's) for the rows of a team from `row` on to hi; two sets
-// of registers in turn.
+// step(row, its data) for every teams-th row from `row` on, with load(data, row) a row ahead; two
+// sets of registers in turn.
 template <typename ROW, typename LOAD, typename STEP>
 __device__ __forceinline__ void for_rows(long row, long hi, int teams, LOAD load, STEP step) {
     ROW one, two;
@@ -368,7 +371,7 @@ __device__ __forceinline__ void for_rows(long row, long hi, int teams, LOAD load
 }
 
 // ---- forward ------------------------------------------------------------------------------
-// OWN: a gate row for each row.  The next row is loaded while this one is worked on.
+// OWN: a gate row for each row.
 template <typename YT, typename XT, bool OWN, int MODE>
 struct FwdRow {
     Raw<YT, MODE> y, gate;
@@ -459,10 +462,11 @@ struct BwdRow {
     float py, ry, ph, rh;   // mean and rstd of y and of h
 };
 
-// OWN: a gate row for each row.  The next row is loaded while this one is worked on.  Workgroups
-// of more than 512 threads have 128 registers a thread: they keep the parameters in LDS and load
-// no row ahead (4000 x 8192 bf16: 117 us; with the parameters in registers 127, with the row
-// ahead and spilled registers 137, with a gate per row 177 against 253).
+// Workgroups of more than 512 threads have 128 registers a thread: they keep the parameters in
+// LDS, load no row ahead and leave the stores their branches (4000 x 8192 bf16 with a gate per row:
+// 132 us; with all registers spilled that these cost 204).  In other workgroups the gate alone is
+// taken again behind the sum, and bf16 is held to three waves a SIMD (10000 x 1400 with a gate per
+// row 63 us, with two 72).
 template <typename YT, typename XT, bool OWN, int TEAM, int MODE>
 __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM,
                              TEAM == 512 && sizeof(XT) == 2 ? 3 : 1) void rnorm_bwd_kernel(RnBwd a) {
@@ -835,8 +839,8 @@ static BwdGeom bwd_geom(const pe_rnorm_desc& d) {
     if (rows < 1) rows = 1;
     g.rows_blk = rows;
     // One workgroup and no fold while its rows cost less: 4 for each team inside a wave (32 x 256:
-    // 8.7 us; 33 rows by items and fold 9.0, and a launch more for the host), 2 for a workgroup
-    // (2 x 4096: 8.0, 4 rows 11.9; 5 rows by items 8.4), 1 past 4096 channels.
+    // 7.5 us; 33 rows by items and fold 8.4, and a launch more for the host), 2 for a workgroup
+    // (2 x 4096: 7.1; by items 4 rows 8.4), 1 past 4096 channels.
     const int team = team_of(d.C);
     g.direct = !grouped && d.rows <= (in_wave(team) ? 4 * at_once : team == 512 ? 2 : 1);
     if (g.direct) g.rows_blk = d.rows;
