@@ -670,7 +670,8 @@ int32_t pe_mul_f32(float* a, const float* b, int64_t n, pe_stream_t stream);
  * Replaces: the batch-norm layers of nets/mobilenet_v2.py (PoseEstimation.pyproj:32; absent).
  *   stats : mean/var (biased) of z per channel -> mean, rstd = 1/sqrt(var+eps),
  *           scale = gamma*rstd, shift = beta - mean*scale; running buffers (may be NULL)
- *           move by `momentum` towards (mean, unbiased var).
+ *           move by `momentum` towards (mean, unbiased var); the pair of a channel whose batch
+ *           mean or variance is not finite stays as it was.
  *   apply : y = act( z*scale + shift (+ residual) ) in bf16; relu 0: none, 1: ReLU, 2: ReLU6.
  *   bwd   : g = da masked by (a > 0) (relu = 1) or (0 < a < 6) (relu = 2) when a != NULL;
  *           dbeta = sum g; dgamma = sum g*xhat;

@@ -49,7 +49,8 @@ DEFAULTS: Dict[str, Dict[str, Any]] = {
                       "params": {"beta1": 0.9, "beta2": 0.999, "epsilon": "1e-8"}},
         # limit of the gradients' global norm over all parameters (None: no clipping), and whether
         # a step whose norm is not finite leaves parameters and moments as they are (the step
-        # counts all the same, and its forward pass has moved the running statistics)
+        # counts all the same; its forward pass has moved the running statistics of the channels
+        # whose batch statistics were finite, and of no other)
         "gradient_clip_norm": None,
         "skip_nonfinite_steps": False,
         "preprocess": {"image_resize": [256, 192]},

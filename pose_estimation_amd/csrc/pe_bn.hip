@@ -216,6 +216,19 @@ struct BnFwdOut {
     float *mean, *rstd, *scale, *shift, *running_mean, *running_var;
 };
 
+// A channel's running pair moves towards the batch's.  A batch mean or variance that is not finite
+// moves neither: NaN would stay in the pair for good, also where the training step is skipped, and
+// fmaxf(var, 0) makes 0 of it, so the variance is tested before that.
+__device__ __forceinline__ void move_running(const BnFwdOut& o, int c, float rm, float rv, float mean,
+                                             float raw_var, float var, float unbias, float momentum) {
+    const float m = (1.0f - momentum) * rm + momentum * mean;
+    const float v = (1.0f - momentum) * rv + momentum * (var * unbias);
+    if (isfinite(raw_var) && isfinite(m) && isfinite(v)) {
+        o.running_mean[c] = m;
+        o.running_var[c] = v;
+    }
+}
+
 __global__ __launch_bounds__(256) void bn_fwd_finalize_kernel(const float* __restrict__ partial,
                                                               int nblk, int C, float inv_m,
                                                               float unbias, const float* gamma,
@@ -230,18 +243,15 @@ __global__ __launch_bounds__(256) void bn_fwd_finalize_kernel(const float* __res
     const int c = fold_partials(partial, nblk, C, s1, s2);
     if (c >= 0) {   // c == cp for the threads that get here
         const float mean = s1 * inv_m;
-        float var = s2 * inv_m - mean * mean;
-        var = fmaxf(var, 0.0f);
+        const float raw_var = s2 * inv_m - mean * mean;
+        const float var = fmaxf(raw_var, 0.0f);
         const float rstd = 1.0f / sqrtf(var + eps);
         const float sc = ga * rstd;
         o.mean[c] = mean;
         o.rstd[c] = rstd;
         o.scale[c] = sc;
         o.shift[c] = be - mean * sc;
-        if (o.running_mean) {
-            o.running_mean[c] = (1.0f - momentum) * rm + momentum * mean;
-            o.running_var[c] = (1.0f - momentum) * rv + momentum * (var * unbias);
-        }
+        if (o.running_mean) move_running(o, c, rm, rv, mean, raw_var, var, unbias, momentum);
     }
 }
 
@@ -457,8 +467,8 @@ __global__ __launch_bounds__(256) void bn_fwd_fused_kernel(
         const int c = fold_partials(partial, nblk, C, s1, s2);
         if (c >= 0) {
             const float mean = s1 * inv_m;
-            float var = s2 * inv_m - mean * mean;
-            var = fmaxf(var, 0.0f);
+            const float raw_var = s2 * inv_m - mean * mean;
+            const float var = fmaxf(raw_var, 0.0f);
             const float rstd = 1.0f / sqrtf(var + eps);
             const float sc = gamma[c] * rstd;
             // the four rows may share cache lines (small C): every store to a line that holds
@@ -467,10 +477,8 @@ __global__ __launch_bounds__(256) void bn_fwd_fused_kernel(
             publish_f32(o.rstd + c, rstd);
             publish_f32(o.scale + c, sc);
             publish_f32(o.shift + c, beta[c] - mean * sc);
-            if (o.running_mean) {
-                o.running_mean[c] = (1.0f - momentum) * o.running_mean[c] + momentum * mean;
-                o.running_var[c] = (1.0f - momentum) * o.running_var[c] + momentum * (var * unbias);
-            }
+            if (o.running_mean)
+                move_running(o, c, o.running_mean[c], o.running_var[c], mean, raw_var, var, unbias, momentum);
         }
         signal_fold_done(sync);
         return;

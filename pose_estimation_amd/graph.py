@@ -658,7 +658,8 @@ class TrainGraph:
         """clip_norm: limit of the gradients' global norm, taken after the exchange, so that every
         rank clips alike; self.grad_norm is then the norm before clipping ([1], on the device).
         skip_nonfinite: leave parameters and moments as they are when that norm is not
-        finite (the step still counts, and running statistics have moved in its forward pass)."""
+        finite (the step still counts, and its forward pass has moved the running statistics of
+        the channels whose batch statistics were finite)."""
         scale = 1.0
         if self.bucketer is not None:
             self.bucketer.finish()

@@ -519,7 +519,8 @@ class TrainablePoseResNet(PoseResNet):
         clip_norm: limit of the gradients' global norm, taken after the exchange, so that every
         rank clips alike; self.grad_norm is then the norm before clipping ([1], on the device).
         skip_nonfinite: leave parameters and moments as they are when that norm is not finite
-        (the step still counts, and running statistics have moved in its forward pass).
+        (the step still counts, and its forward pass has moved the running statistics of the
+        channels whose batch statistics were finite).
         Returns (loss [1] float32 device tensor, per_joint [K])."""
         if host_replay:
             loss, per_joint = self.replay_host(self._pass, images_u8, x_s2d, joints, mask)
