@@ -462,10 +462,11 @@ class GradSet:
     strides (the gradient itself allowed); None: in place.
 
     The set keeps the tensors and reads their values anew at every call, so a program builds it
-    once over the gradients that every step refills in place.  It can be used on any stream of
-    its device, by several at a time, and in a captured graph, which it has to outlive.  The
-    tensors must stay in place: not resized, not given other memory.  Tensors that share memory with
-    one another are refused: they would count twice, and be scaled twice."""
+    once over the gradients that every step refills in place.  Building it waits for the work
+    of the current stream, because its table is copied from the host.  It can be used on any
+    stream of its device, by several at a time, and in a captured graph, which it has to outlive.
+    The tensors must stay in place: not resized, not given other memory.  Tensors that share
+    memory with one another are refused: they would count twice, and be scaled twice."""
 
     _SPAN = np.dtype([("src", np.uint64), ("dst", np.uint64), ("n", np.int64),
                       ("dtype", np.int32), ("reserved", np.int32)])
@@ -473,7 +474,7 @@ class GradSet:
     MIN_SHARE, START = 8192, 1024
 
     def __init__(self, tensors: Sequence[torch.Tensor],
-                 out: Optional[Sequence[torch.Tensor]] = None):
+                 out: Optional[Sequence[torch.Tensor]] = None, *, _one_call: bool = False):
         self.tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
         if not self.tensors:
             raise ValueError("a GradSet needs at least one tensor")
@@ -512,14 +513,15 @@ class GradSet:
             raise RuntimeError("build the GradSet before the capture: its table is copied from "
                                "the host")
         with torch.cuda.device(self.device):
-            self._table, self.shares = self._cut(spans)
+            self._table, self.shares = self._cut(spans, _one_call)
             self._stream = _stream(self._table)
         self._begin = self._table.data_ptr() + self._spans * self._SPAN.itemsize
 
-    def _cut(self, spans):
+    def _cut(self, spans, one_call: bool = False):
         """(table on the device, number of shares).  The tensors lie end to end on a line, each
         with START idle bytes behind it; a share is what lies between two of its equal marks, so
-        spans start at 16-byte steps of their tensor."""
+        spans start at 16-byte steps of their tensor.  one_call: the table is for the current
+        stream alone, so it need not have arrived when this returns."""
         if not spans:
             self._spans = 0
             return torch.zeros(1, dtype=torch.int32, device=self.device), 0
@@ -540,8 +542,14 @@ class GradSet:
         shares = int(k[-1]) + 1
         begin = np.searchsorted(k, np.arange(shares + 1)).astype(np.int32)
         self._spans = len(rows)
-        packed = np.frombuffer(rows.tobytes() + begin.tobytes(), np.uint8).copy()
-        return torch.from_numpy(packed).to(self.device), shares
+        packed = np.frombuffer(rows.tobytes() + begin.tobytes(), np.uint8)
+        if not one_call:
+            return torch.from_numpy(packed.copy()).to(self.device), shares
+        # pinned: the allocator hands the buffer out again only after the copy
+        staged = torch.empty(packed.size, dtype=torch.uint8, pin_memory=True)
+        staged.numpy()[:] = packed
+        table = torch.empty(packed.size, dtype=torch.uint8, device=self.device)
+        return table.copy_(staged, non_blocking=True), shares
 
     def _on_stream(self):
         """(spans, begin, shares) for a launch on the device's current stream.  The allocator is
@@ -557,7 +565,7 @@ class GradSet:
 
 
 def _as_set(grads) -> GradSet:
-    return grads if isinstance(grads, GradSet) else GradSet(grads)
+    return grads if isinstance(grads, GradSet) else GradSet(grads, _one_call=True)
 
 
 def grad_norm(grads, norm_type: float = 2.0, grad_scale: float = 1.0,
@@ -565,7 +573,8 @@ def grad_norm(grads, norm_type: float = 2.0, grad_scale: float = 1.0,
               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Global norm of grad_scale * every gradient -> [1] float32 on the device (no host sync).
 
-    grads: a GradSet, or a tensor or sequence of tensors, for which a set is made for this call.
+    grads: a GradSet, or a tensor or sequence of tensors, for which a set is made for this call
+    (host work for every tensor; its table is copied without waiting for the device).
     norm_type: 2 (squares summed in float64) or inf (the largest magnitude).  NaN and infinities
     carry over to the norm."""
     s = _as_set(grads)
@@ -583,9 +592,9 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, grad_scale: float
                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """g * grad_scale * min(1, max_norm / norm) for every gradient of the set, in place or into
     the set's `out`, rounded once; norm = grad_norm(grads, norm_type, grad_scale), returned as
-    [1] float32 on the device (in `out` if given).  A norm that is not finite makes every result
-    NaN, as TensorFlow's clip_by_global_norm does, the framework of the reference
-    (test.ipynb:19); there is no epsilon, so a norm within the limit changes no bit."""
+    [1] float32 on the device (in `out` if given).  grads: as there.  A norm that is not finite
+    makes every result NaN, as TensorFlow's clip_by_global_norm does, the framework of the
+    reference (test.ipynb:19); there is no epsilon, so a norm within the limit changes no bit."""
     s = _as_set(grads)
     kind = _norm_kind(norm_type)
     max_norm = float(max_norm)

@@ -550,3 +550,46 @@ def test_tape_graph_networks_take_the_limit(family):
     pe.clip_grads(pe.GradSet([t.net.grads], out=[clipped]), 1e-3)
     pe.adam_step(before, torch.zeros_like(before), torch.zeros_like(before), clipped, 1, 1e-3)
     assert torch.equal(before, t.net.master)
+
+
+@gpu
+def test_lists_are_taken_without_waiting_for_the_device():
+    """grad_norm and clip_grads of a plain list return while work queued before them still runs;
+    several lists in a row, each with a table of its own."""
+    gen = seeded(14)
+    lists = [[rand(gen, n + 16 * k) for n in (50_000, 7, 3001)] for k in range(6)]
+    want = [norm64(g) for g in lists]
+    for _ in range(2):                     # the staging memory is there
+        for g in lists:
+            pe.grad_norm(g), pe.clip_grads(g, INF)
+    a = torch.randn(8192, 8192, device="cuda").bfloat16()
+    b = torch.mm(a, a)
+    torch.cuda.synchronize()
+    for _ in range(300):                   # about 0.3 s
+        torch.mm(a, a, out=b)
+    done = torch.cuda.Event()
+    done.record()
+    norms = [pe.grad_norm(g) for g in lists]
+    clipped = [pe.clip_grads(g, 0.5 * n) for g, n in zip(lists, want)]
+    assert not done.query()
+    torch.cuda.synchronize()
+    for n, c, g, w in zip(norms, clipped, lists, want):
+        assert_norm(n, w)
+        assert_norm(c, w)
+        # every element rounded by at most half a step, so the norm of the results as well
+        assert abs(norm64(g) - 0.5 * w) <= 2 * U32 * w
+
+
+@gpu
+def test_a_recorded_call_list_repeats_calls_on_lists():
+    from pose_estimation_amd import replay
+
+    def work(x):
+        g = x.clone()
+        return pe.grad_norm([g, x]), pe.clip_grads([g], 1.0), g
+
+    rec = replay.RecordedPass(work, [rand(seeded(4), 70_001)], torch.device("cuda", 0))
+    for seed in (5, 6, 7):
+        x = rand(seeded(seed), 70_001)
+        for a, b in zip([t.clone() for t in rec(x)], work(x)):
+            assert torch.equal(a, b)
