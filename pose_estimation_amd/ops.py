@@ -3,6 +3,7 @@ and for the current HIP stream; all arithmetic happens in libpe_hip.so.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
 import math
 from typing import Optional, Sequence, Tuple
@@ -325,7 +326,8 @@ def adam_scalars(lr: float, beta1: float, beta2: float, step: int, tf1: bool = T
 
 
 def _clip_desc(max_norm: float, norm_type: float, grad_scale: float, skip_nonfinite: bool,
-               norm_over: Optional["GradSet"], like: torch.Tensor) -> ClipDesc:
+               norm_over: Optional["GradSet"], like: torch.Tensor,
+               grad: torch.Tensor) -> ClipDesc:
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
@@ -334,6 +336,8 @@ def _clip_desc(max_norm: float, norm_type: float, grad_scale: float, skip_nonfin
                         int(bool(skip_nonfinite)))
     if norm_over.device != like.device:
         raise ValueError(f"norm_over is on {norm_over.device}, the parameters on {like.device}")
+    if grad.numel() and not norm_over._holds(grad):
+        raise ValueError("norm_over does not hold the gradients of this step")
     spans, begin, shares = norm_over._on_stream()
     return ClipDesc(spans, begin, max_norm, shares, _norm_kind(norm_type), grad_scale,
                     int(bool(skip_nonfinite)))
@@ -349,10 +353,10 @@ def adam_step(p: torch.Tensor, m: torch.Tensor, v: torch.Tensor, grad: torch.Ten
 
     max_norm: clip the gradients (times grad_scale) to this global norm inside the step, which
     leaves `grad` as it is, and return the norm before clipping, [1] float32 on the device.
-    The norm is taken over `grad`, or over `norm_over`, a GradSet, where the arena is only a
-    part of what is clipped together.  A norm that is not finite makes every parameter NaN, or
-    with skip_nonfinite leaves p, m, v and p_bf16 untouched (`step` is the caller's count);
-    max_norm = inf only skips."""
+    The norm is taken over `grad`, or over `norm_over`, a GradSet that holds `grad` (or tensors
+    inside it) among others, where the arena is only a part of what is clipped together.  A norm
+    that is not finite makes every parameter NaN, or with skip_nonfinite leaves p, m, v and
+    p_bf16 untouched (`step` is the caller's count); max_norm = inf only skips."""
     _need_gpu(p, m, v, grad, p_bf16)
     for t in (p, m, v, grad):
         if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != p.numel():
@@ -362,7 +366,7 @@ def adam_step(p: torch.Tensor, m: torch.Tensor, v: torch.Tensor, grad: torch.Ten
         raise ValueError("p_bf16 must be contiguous bfloat16 of the same length")
     s, a = adam_scalars(lr, beta1, beta2, step, tf1)
     if max_norm is not None:
-        d = _clip_desc(max_norm, norm_type, grad_scale, skip_nonfinite, norm_over, p)
+        d = _clip_desc(max_norm, norm_type, grad_scale, skip_nonfinite, norm_over, p, grad)
         norm, workspace, ws = _norm_buffers(p.device, None, workspace, norm_over is None and
                                             p.numel() <= PE_NORM_FEW_ELEMENTS)
         with on_device(p):
@@ -397,7 +401,7 @@ def sgd_step(p: torch.Tensor, mom: torch.Tensor, grad: torch.Tensor, lr: float,
         if p_bf16 is not None and (p_bf16.dtype != torch.bfloat16 or not p_bf16.is_contiguous()
                                    or p_bf16.numel() != p.numel()):
             raise ValueError("p_bf16 must be contiguous bfloat16 of the same length")
-        d = _clip_desc(max_norm, norm_type, grad_scale, skip_nonfinite, norm_over, p)
+        d = _clip_desc(max_norm, norm_type, grad_scale, skip_nonfinite, norm_over, p, grad)
         norm, workspace, ws = _norm_buffers(p.device, None, workspace, norm_over is None and
                                             p.numel() <= PE_NORM_FEW_ELEMENTS)
         with on_device(p):
@@ -485,7 +489,7 @@ class GradSet:
         _need_gpu(*self.tensors, *self.out)
         self.device = self.tensors[0].device
         self.numel = 0
-        spans, ranges = [], []
+        spans, ranges, self._ranges = [], [], []
         for t, o in zip(self.tensors, self.out):
             if t.device != self.device or o.device != self.device:
                 raise ValueError("the tensors of a GradSet are on one device")
@@ -503,10 +507,11 @@ class GradSet:
             self.numel += n
             src, dst = t.data_ptr(), o.data_ptr()
             spans.append((src, dst, n, size))
-            ranges.append((src, src + n * size))
+            self._ranges.append((src, src + n * size))
             if dst != src:
                 ranges.append((dst, dst + n * size))
-        ranges.sort()
+        self._ranges.sort()
+        ranges = sorted(self._ranges + ranges)
         if any(a[1] > b[0] for a, b in zip(ranges, ranges[1:])):
             raise ValueError("tensors of a GradSet share memory")
         if torch.cuda.is_current_stream_capturing():
@@ -559,6 +564,13 @@ class GradSet:
                 not torch.cuda.is_current_stream_capturing():
             self._table.record_stream(torch.cuda.current_stream(self.device))
         return self._table.data_ptr(), self._begin, self.shares
+
+    def _holds(self, t: torch.Tensor) -> bool:
+        """Whether a gradient of the set lies in the memory of t (contiguous)."""
+        lo = t.data_ptr()
+        hi = lo + t.numel() * t.element_size()
+        k = bisect.bisect_left(self._ranges, (hi, 0))   # what starts before the end of t
+        return hi > lo and k > 0 and self._ranges[k - 1][1] > lo
 
     def __len__(self) -> int:
         return len(self.tensors)

@@ -593,3 +593,36 @@ def test_a_recorded_call_list_repeats_calls_on_lists():
         x = rand(seeded(seed), 70_001)
         for a, b in zip([t.clone() for t in rec(x)], work(x)):
             assert torch.equal(a, b)
+
+
+def test_a_set_knows_whether_it_holds_an_arena():
+    s = object.__new__(ops.GradSet)
+    v = torch.zeros(100)
+    at = v.data_ptr()
+    s._ranges = [(at + 40, at + 80), (at + 200, at + 240)]
+    for lo, hi, held in ((0, 10, False), (0, 11, True), (12, 13, True), (19, 20, True),
+                         (20, 50, False), (20, 51, True), (59, 100, True), (60, 100, False),
+                         (0, 100, True), (5, 5, False)):
+        assert s._holds(v[lo:hi]) is held, (lo, hi)
+    s._ranges = []
+    assert s._holds(v) is False
+
+
+@gpu
+def test_a_norm_over_other_tensors_is_refused():
+    """The norm a step is clipped by has the step's own gradients in it."""
+    p, m, v, g, _ = arenas(3000, 4)
+    other = rand(seeded(8), 3000)
+    before = [t.clone() for t in (p, m, v)]
+    with pytest.raises(ValueError, match="norm_over"):
+        pe.adam_step(p, m, v, g, 1, max_norm=1.0, norm_over=pe.GradSet([other]))
+    with pytest.raises(ValueError, match="norm_over"):
+        pe.sgd_step(p, m, g, 0.1, max_norm=1.0, norm_over=pe.GradSet([other]))
+    for a, b in zip((p, m, v), before):
+        assert torch.equal(a, b)
+    parts = pe.GradSet([other, g[1000:2000]])       # the tensors of an arena with gaps
+    assert_norm(pe.sgd_step(p, m, g, 0.1, max_norm=1.0, norm_over=parts),
+                norm64([other, g[1000:2000]]))
+    none = torch.empty(0, device="cuda")
+    assert_norm(pe.sgd_step(none, none, none, 0.1, max_norm=1.0, norm_over=pe.GradSet([other])),
+                norm64([other]))
