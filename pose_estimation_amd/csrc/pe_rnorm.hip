@@ -234,7 +234,7 @@ __device__ __forceinline__ float dot8(f32x8 own_v, f32x8 w, const Cols<MODE>& k)
 // one barrier a sum is enough.
 struct TeamSums {
     float2* buf;    // LDS [2][16], workgroup teams only
-    int waves, turn;
+    int wave, waves, turn;
     // 1 / this wave's channels, and the channels of the wave of the lane's index; forward only
     float per_wave, in_lane;
 };
@@ -245,7 +245,7 @@ __host__ __device__ constexpr int waves_of(int C) { return (C + 64 * kRnEl - 1) 
 __device__ __forceinline__ float2 each_wave(float2 v, TeamSums& ts) {
     float2* buf = ts.buf + 16 * ts.turn;
     ts.turn ^= 1;
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) buf[ts.wave] = v;
     __syncthreads();
     const int w = (int)threadIdx.x & 15;
     v = buf[w];
@@ -301,22 +301,21 @@ __device__ __forceinline__ float as_float(T v) {
     return sizeof(T) == 4 ? (float)v : bf16_bits_to_float((uint32_t)v);
 }
 
-__device__ __forceinline__ float sigmoid(float g) {
-    return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
-}
-
-// phi(g) and, with a derivative, phi'(g).
+// phi(g) and, with a derivative, phi'(g), from s = sigmoid(g) and c = 1 - s = exp(-g) s: the
+// difference would lose what is left of c where s is near 1 (all of it from g = 17 on).
 __device__ __forceinline__ float gate_value(float g, int act, float& slope) {
     if (act == PE_GATE_NONE) {
         slope = 1.0f;
         return g;
     }
-    const float s = sigmoid(g);
+    const float e = __expf(-g);
+    const float s = __builtin_amdgcn_rcpf(1.0f + e);
+    const float c = fminf(e, FLT_MAX) * s;   // 0, not NaN, where s has vanished
     if (act == PE_GATE_SIGMOID) {
-        slope = s * (1.0f - s);
+        slope = s * c;
         return s;
     }
-    slope = s * (1.0f + g * (1.0f - s));
+    slope = __builtin_fmaf(g * s, c, s);
     return g * s;
 }
 
@@ -389,7 +388,7 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_k
         const int n = a.C - wave * 64 * kRnEl;
         return (float)(n < 0 ? 0 : n < 64 * kRnEl ? n : 64 * kRnEl);
     };
-    TeamSums ts{lds, waves_of(a.C), 0, 0.0f, 0.0f};
+    TeamSums ts{lds, (int)threadIdx.x >> 6, waves_of(a.C), 0, 0.0f, 0.0f};
     if (!in_wave(TEAM)) {
         ts.per_wave = 1.0f / channels_of((int)threadIdx.x >> 6);
         ts.in_lane = channels_of((int)threadIdx.x & 15);
@@ -472,12 +471,15 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM,
                              TEAM == 512 && sizeof(XT) == 2 ? 3 : 1) void rnorm_bwd_kernel(RnBwd a) {
     __shared__ float2 lds[in_wave(TEAM) ? 1 : 32];
     __shared__ float fold[in_wave(TEAM) ? kRnThreads / 64 : 1][4][in_wave(TEAM) ? TEAM * kRnEl : 1];
-    TeamSums ts{lds, waves_of(a.C), 0, 0.0f, 0.0f};
+    constexpr bool WIDE = TEAM == 1024, ALL = !WIDE && store_all(TEAM, MODE);
+    // The wave's number as the scalar it is where a register of each thread is one too many
+    // (10000 x 1400 bf16 with a gate per row 60 us, with a reload in the loop 70).
+    const int wave = OWN && !WIDE ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : (int)threadIdx.x >> 6;
+    TeamSums ts{lds, wave, waves_of(a.C), 0, 0.0f, 0.0f};
     const int T = team_size<TEAM>();
     const int t = in_wave(TEAM) ? (int)threadIdx.x % T : (int)threadIdx.x;
     const int teams = in_wave(TEAM) ? kRnThreads / T : 1;
     const Cols<MODE> k(t, a.C);
-    constexpr bool WIDE = TEAM == 1024, ALL = !WIDE && store_all(TEAM, MODE);
     __shared__ f32x4 held[WIDE ? 6 : 1][WIDE ? 1024 : 1];   // each thread's own, no barrier
     const f32x8 s = load_param<MODE>(a.s, 1.0f, k);
     f32x8 A = load_param<MODE>(a.gp, 1.0f, k) * s;

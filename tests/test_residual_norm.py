@@ -800,3 +800,31 @@ def test_a_block_of_a_network_trained_with_a_clipped_norm():
             torch.testing.assert_close(a, b, rtol=4 * U, atol=1e-12)
         norms.append(float(norm))
     assert all(np.isfinite(norms)) and bool(master.isfinite().all())
+
+
+@gpu
+@pytest.mark.parametrize("types", ["bf16", "f32"])
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+@pytest.mark.parametrize("gate,rows,groups", [("row", 3, 0), ("group", 4, 2)])
+@pytest.mark.parametrize("C", [61, 1040, 4203])
+def test_slopes_of_saturated_gates(types, act, gate, rows, groups, C):
+    """dgate = phi'(gate) itself (y = dh = 1, nothing else) for gates from -30 to 30, within a bound
+    relative to the slope's terms s and 1 - s, which are both tiny on one side.
+
+    exp's argument is rounded (2|g| steps of relative error with the constant's), exp, the reciprocal
+    and each sum and product add at most two steps: (2|g| + 12) U in s and in 1 - s each.  The sums
+    over a group's rows, in which every term is the same, are exact or rounded by one step."""
+    yt = TYPES[types][0]
+    g = torch.linspace(-30, 30, C, device="cuda").to(yt)
+    count = groups or rows
+    gates = torch.stack([g.roll(k) for k in range(count)])
+    y = torch.ones(rows, C, dtype=yt, device="cuda")
+    got = nn.residual_norm_bwd(torch.ones_like(y), None, y, None, None, gate=gates, gate_act=act)["dgate"]
+    g64 = gates.double()
+    s, c = torch.sigmoid(g64), torch.sigmoid(-g64)
+    want = s * c if act == "sigmoid" else s * (1 + g64 * c)
+    terms = s * c if act == "sigmoid" else s * (1 + g64.abs() * c)
+    per = rows // groups if groups else 1
+    bound = per * ((4 * g64.abs() + 26) * U * terms) * (1 + HALF_STEP[yt]) + HALF_STEP[yt] * per * want.abs()
+    off = (got.double() - per * want).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())
