@@ -65,6 +65,7 @@ struct RnBwd {
     long rows, gate_rows;
     long lddh, lddz, ldy, ldx, ldg, lddy, lddx, lddg;
     long group, nseg, rows_blk;   // rows of a group, items of a group, rows of an item
+    long first;                   // item of the grid's first workgroup
     float inv_c;
     int C, pre, post, layer, act;
 };
@@ -495,8 +496,9 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM,
         v.hi = held[2 * i + 1][threadIdx.x];
         return v;
     };
-    const long g = (long)blockIdx.x / a.nseg;
-    const long lo = g * a.group + ((long)blockIdx.x - g * a.nseg) * a.rows_blk;
+    const long item = a.first + blockIdx.x;
+    const long g = item / a.nseg;
+    const long lo = g * a.group + (item - g * a.nseg) * a.rows_blk;
     const long end = (g + 1) * a.group;
     const long hi = lo + a.rows_blk < end ? lo + a.rows_blk : end;
     const bool shared = !OWN && a.gate_rows;
@@ -591,7 +593,7 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM,
     }
     if (!a.need) return;
     const bool direct = a.part == nullptr;
-    float* out = direct ? nullptr : a.part + (long)blockIdx.x * slots_of(a.gate_rows) * a.pitch;
+    float* out = direct ? nullptr : a.part + item * slots_of(a.gate_rows) * a.pitch;
     if (in_wave(TEAM)) {
         // rows side by side in the wave, then the waves in order
 #pragma unroll
@@ -912,18 +914,24 @@ template <typename YT, typename XT, bool OWN>
 struct BwdOf {
     template <int TEAM, int MODE>
     struct F {
-        static void go(const RnBwd& a, unsigned blocks, hipStream_t st) {
-            launch(rnorm_bwd_kernel<YT, XT, OWN, TEAM, MODE>, blocks, block_of(a.C), 0, st, a);
+        // A grid holds less than 2^32 threads: short runs of a shared gate take more than one.
+        static void go(RnBwd a, long items, hipStream_t st) {
+            const unsigned threads = block_of(a.C);
+            const long most = 0xffffffffl / threads;
+            for (a.first = 0; a.first < items; a.first += most) {
+                const unsigned blocks = (unsigned)(items - a.first < most ? items - a.first : most);
+                launch(rnorm_bwd_kernel<YT, XT, OWN, TEAM, MODE>, blocks, threads, 0, st, a);
+            }
         }
     };
 };
 
 template <typename YT, typename XT>
-static void launch_bwd(const RnBwd& a, unsigned blocks, hipStream_t st) {
+static void launch_bwd(const RnBwd& a, long items, hipStream_t st) {
     if (a.gate_rows == 1) {
-        with_team<BwdOf<YT, XT, true>::template F>(a.C, a, blocks, st);
+        with_team<BwdOf<YT, XT, true>::template F>(a.C, a, items, st);
     } else {
-        with_team<BwdOf<YT, XT, false>::template F>(a.C, a, blocks, st);
+        with_team<BwdOf<YT, XT, false>::template F>(a.C, a, items, st);
     }
 }
 
@@ -1091,7 +1099,6 @@ extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const vo
         PE_REQUIRE(!dgate || d->rows == d->gate_rows || d->lddgate >= d->C, PE_E_INVALID,
                    "pe_rnorm_bwd: rows of dgate overlap");
         g = bwd_geom(*d);
-        PE_REQUIRE(g.items() <= 0x7fffffffl, PE_E_UNSUPPORTED, "pe_rnorm_bwd: too many gate rows");
         if (need && !g.direct) {
             PE_REQUIRE(workspace && aligned(workspace, 16), PE_E_INVALID,
                        "pe_rnorm_bwd: workspace must be given, 16-byte aligned");
@@ -1141,7 +1148,7 @@ extern "C" int32_t pe_rnorm_bwd(const pe_rnorm_desc* d, const void* dh, const vo
         a.layer = d->norm == PE_RNORM_LAYER;
         a.act = d->gate_act;
         const int yd = d->y_dtype, xd = d->x_dtype;
-        const unsigned items = (unsigned)g.items();
+        const long items = g.items();
         if (yd == PE_DTYPE_F32) {
             launch_bwd<float, float>(a, items, as_stream(stream));
         } else if (xd == PE_DTYPE_F32) {

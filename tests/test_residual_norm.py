@@ -828,3 +828,39 @@ def test_slopes_of_saturated_gates(types, act, gate, rows, groups, C):
     bound = per * ((4 * g64.abs() + 26) * U * terms) * (1 + HALF_STEP[yt]) + HALF_STEP[yt] * per * want.abs()
     off = (got.double() - per * want).abs()
     assert bool((off <= bound).all()), float((off / bound).max())
+
+
+@gpu
+def test_more_gate_rows_than_a_launch_holds():
+    """17 million runs of two rows, more than the workgroups of 2^32 threads: every output is that
+    of the two halves called apart, and the sum over all rows is one of every row's dz.  An item's
+    sum of two values is rounded once, a slice's sum and the result once more."""
+    groups, C = 17_000_000, 8
+    gen = torch.Generator(device="cuda").manual_seed(6)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=gen, device="cuda")
+
+    t = {k: normal(2 * groups, C).bfloat16() for k in ("y", "x", "dh", "dz")}
+    t.update(gate=normal(groups, C).bfloat16(), scale=normal(C), post=(normal(C), normal(C)),
+             pre=(normal(C), normal(C)))
+
+    def backward(lo, hi):
+        rows = {k: t[k][2 * lo:2 * hi] for k in ("y", "x", "dh", "dz")}
+        kw = dict(norm="layer", post=t["post"], pre=t["pre"], scale=t["scale"], gate=t["gate"][lo:hi],
+                  gate_act="sigmoid")
+        stats = nn.residual_norm(rows["y"], rows["x"], want_stats=True, **kw)[2]
+        return nn.residual_norm_bwd(rows["dh"], rows["dz"], rows["y"], rows["x"], stats, **kw)
+
+    whole = backward(0, groups)
+    half = groups // 2
+    for lo, hi in ((0, half), (half, groups)):
+        part = backward(lo, hi)
+        assert torch.equal(part["dgate"], whole["dgate"][lo:hi])
+        for k in ("dy", "dx"):
+            assert torch.equal(part[k], whole[k][2 * lo:2 * hi]), k
+    each = t["dz"].view(groups, 2, C).float().sum(1)
+    want = each.sum(0, dtype=torch.float64)
+    bound = 4 * U * each.abs().sum(0, dtype=torch.float64)
+    assert bool(((whole["dpre_beta"].double() - want).abs() <= bound).all())
+    assert float(bound.max()) < 10 and all(bool(whole[k].isfinite().all()) for k in whole)
