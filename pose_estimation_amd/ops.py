@@ -551,7 +551,7 @@ class GradSet:
         if not one_call:
             return torch.from_numpy(packed.copy()).to(self.device), shares
         # pinned: the allocator hands the buffer out again only after the copy
-        staged = torch.empty(packed.size, dtype=torch.uint8, pin_memory=True)
+        staged = torch.empty(packed.size, dtype=torch.uint8, device="cpu", pin_memory=True)
         staged.numpy()[:] = packed
         table = torch.empty(packed.size, dtype=torch.uint8, device=self.device)
         return table.copy_(staged, non_blocking=True), shares

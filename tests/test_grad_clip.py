@@ -626,3 +626,11 @@ def test_a_norm_over_other_tensors_is_refused():
     none = torch.empty(0, device="cuda")
     assert_norm(pe.sgd_step(none, none, none, 0.1, max_norm=1.0, norm_over=pe.GradSet([other])),
                 norm64([other]))
+
+
+@gpu
+def test_lists_under_a_default_device():
+    g = [rand(seeded(15), 5000), rand(seeded(16), 9, torch.bfloat16)]
+    with torch.device("cuda"):
+        assert_norm(pe.grad_norm(g), norm64(g))
+        assert_norm(pe.clip_grads(pe.GradSet(g), INF), norm64(g))
