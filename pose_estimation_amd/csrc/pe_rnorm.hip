@@ -13,10 +13,11 @@
 // would not leave a wave the registers to have the next row under way, narrower ones add lanes to
 // every sum.  Where a last wave has little to do (just past 512, 1024, 2048, 4096 channels) the
 // vector instructions bound it instead, about 190 for eight channels forward, 350 backward.
-// Measured: forward 8192 x 4096 bf16 with a float32 residual and a gate per row 88 us (5.3 TB/s),
-// 196608 x 256 bf16 with a gate per image 74 us (5.5 TB/s) and backward there 128 us (4.7 TB/s, as a
-// copy), 8000 x 4096 bf16 46 us (5.7 TB/s) and backward with its fold 88 us (4.5 TB/s), one row of
-// 4096 3.2 us.
+// Measured on the device: forward 8192 x 4096 bf16 with a float32 residual and a gate per row 88 us
+// (5.3 TB/s), 196608 x 256 bf16 with a gate per image 75 us (5.4 TB/s) and backward there 129 us
+// (4.7 TB/s, as a copy), 8000 x 4096 bf16 43 us (6.1 TB/s) and backward with its fold 88 us
+// (4.5 TB/s), one row of 4096 3.2 us.  Where the comments below set two choices side by side, both
+// were timed as calls in a row, one to three us more than the device takes.
 #include <float.h>
 #include <math.h>
 
@@ -231,7 +232,7 @@ __device__ __forceinline__ float dot8(f32x8 own_v, f32x8 w, const Cols<MODE>& k)
 
 // ---- sums over a row's team ---------------------------------------------------------------
 // A workgroup as a team: the waves' values through LDS, then a lane for each of the at most 16
-// waves (with a loop over them instead 4000 x 8192 bf16 took 77 us, not 69); two buffers in turn, so
+// waves (a loop over them instead took 12 % more at 4000 x 8192 bf16); two buffers in turn, so
 // one barrier a sum is enough.
 struct TeamSums {
     float2* buf;    // LDS [2][16], workgroup teams only
@@ -449,8 +450,9 @@ __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM) void rnorm_fwd_k
 //   dx = D;  dy = norm backward of u*s*gp at y;  dgate = phi' * sum_group D*s*(gp*yhat + bp)
 //   dgq = sum dz*hhat, dbq = sum dz, dgp = s * sum u*yhat, dbp = s * sum u,
 //   ds = gp * sum u*yhat + bp * sum u
-// h is rebuilt in float32 from x and y, exactly as forward had it before rounding: the same bytes
-// as reading the stored h, without its rounding in the gradients.  Four sums a channel stay in
+// h is rebuilt in float32 from x and y, as forward had it before its rounding (with a gate shared by
+// rows up to float32 roundings: phi is multiplied into the parameters here, once an item): the same
+// bytes as reading the stored h, without its rounding in the gradients.  Four sums a channel stay in
 // registers over an item's rows and go to the workspace once an item; a second launch folds the
 // items in order in float64, so the results have the same bits on every call.  An item never
 // crosses a gate row: phi is a constant of the item, which leaves its sums of D with phi (for the
@@ -466,7 +468,7 @@ struct BwdRow {
 // LDS, load no row ahead and leave the stores their branches (4000 x 8192 bf16 with a gate per row:
 // 132 us; with all registers spilled that these cost 204).  In other workgroups the gate alone is
 // taken again behind the sum, and bf16 is held to three waves a SIMD (10000 x 1400 with a gate per
-// row 63 us, with two 72).
+// row 63 us when that was chosen, with two 72).
 template <typename YT, typename XT, bool OWN, int TEAM, int MODE>
 __global__ __launch_bounds__(in_wave(TEAM) ? kRnThreads : TEAM,
                              TEAM == 512 && sizeof(XT) == 2 ? 3 : 1) void rnorm_bwd_kernel(RnBwd a) {
